@@ -40,6 +40,18 @@ void launch_attn_extend(const void* q, int64_t q_stride, const void* k_cache, co
                         int64_t out_stride, int B, int max_qlen, int nh, int nkv, int D, int bs, float scale,
                         hipStream_t st, bool kv8, void* q8, void* s8, int window, int nsplit, int split_keys,
                         void* part_o, void* part_ml, int total);
+int attn_shared_parts(int T, int B, int nh, int nkv, int D, int P, int max_qlen, int max_own);
+void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const void* vc, int pages, const void* prefix_table, int P,
+                        const void* bt, int64_t bt_stride, int bt_width, const void* cu, const void* ctx, void* out, int64_t out_stride,
+                        void* ws, int parts, int T, int B, int nh, int nkv, int D, int bs, int max_qlen, int max_own, float scale,
+                        bool kv8, hipStream_t st);
+void launch_adjust_logits(const void* x, int64_t ldx, bool x32, void* y, int64_t ldy, bool y32, int B, int V, const void* ids, int64_t ldi,
+                          int most, bool ids64, const void* lens, const void* prompts, const void* rep, const void* pres,
+                          const void* freq, const void* bias_ids, const void* bias, int64_t ldb, int biases, const void* mask,
+                          int64_t ldm, const void* mask_rows, int masks, hipStream_t st);
+int logprobs_runs(int B, int V, int n);
+void launch_logprobs(const void* logits, int64_t ld, bool fp32, const void* tokens, int B, int V, int n, void* part, void* top, void* lp,
+                     void* rank, void* top_ids, void* top_lp, hipStream_t st);
 bool attn_extend_two(int total, int B, int max_qlen, int nh, int nkv, int D);
 int launch_gemm_qkv_args(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, void* y, int64_t ldy,
                          int M, int N, int K, void* workspace, int64_t ws_bytes, int nt_hint, int split_hint,
@@ -342,6 +354,25 @@ PYBIND11_MODULE(_C, m) {
      pybind11::arg("bs"), pybind11::arg("scale"), pybind11::arg("st"), pybind11::arg("kv8"), pybind11::arg("q8") = 0,
      pybind11::arg("s8") = 0, pybind11::arg("window") = 0, pybind11::arg("nsplit") = 1,
      pybind11::arg("split_keys") = 0, pybind11::arg("po") = 0, pybind11::arg("pml") = 0, pybind11::arg("total") = 0);
+  m.def("attn_shared_parts", &attn_shared_parts);  // (rows, sequences, heads, kv heads, head dim, prefix, longest portion, own part)
+  m.def("attn_shared", [](uintptr_t q, int64_t qs, uintptr_t kc, uintptr_t vc, int pages, uintptr_t ptab, int P_, uintptr_t bt, int64_t bts,
+                          int btw, uintptr_t cu, uintptr_t ctx, uintptr_t out, int64_t os, uintptr_t ws, int parts, int T, int B, int nh,
+                          int nkv, int D, int bs, int maxq, int maxo, float scale, bool kv8, uintptr_t st) {
+    launch_attn_shared(CP(q), qs, CP(kc), CP(vc), pages, CP(ptab), P_, CP(bt), bts, btw, CP(cu), CP(ctx), P(out), os, P(ws), parts, T, B,
+                       nh, nkv, D, bs, maxq, maxo, scale, kv8, S(st));
+  });
+  m.def("adjust_logits", [](uintptr_t x, int64_t ldx, bool x32, uintptr_t y, int64_t ldy, bool y32, int B, int V, uintptr_t ids, int64_t ldi,
+                            int most, bool ids64, uintptr_t lens, uintptr_t prompts, uintptr_t rep, uintptr_t pres, uintptr_t freq,
+                            uintptr_t bids, uintptr_t bias, int64_t ldb, int nb, uintptr_t mask, int64_t ldm, uintptr_t mrows, int masks,
+                            uintptr_t st) {
+    launch_adjust_logits(CP(x), ldx, x32, P(y), ldy, y32, B, V, CP(ids), ldi, most, ids64, CP(lens), CP(prompts), CP(rep), CP(pres),
+                         CP(freq), CP(bids), CP(bias), ldb, nb, CP(mask), ldm, CP(mrows), masks, S(st));
+  });
+  m.def("logprobs_runs", &logprobs_runs);  // (rows, vocabulary, likeliest tokens asked for)
+  m.def("token_logprobs", [](uintptr_t lg, int64_t ld, bool fp32, uintptr_t tok, int B, int V, int n, uintptr_t part, uintptr_t top,
+                             uintptr_t lp, uintptr_t rank, uintptr_t tid, uintptr_t tlp, uintptr_t st) {
+    launch_logprobs(CP(lg), ld, fp32, CP(tok), B, V, n, P(part), P(top), P(lp), P(rank), P(tid), P(tlp), S(st));
+  });
   m.def("attn_extend_two", &attn_extend_two);  // (total rows, sequences, longest portion, heads, kv heads, head dim)
   m.def("gemm", [](uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw, bool fp8, uintptr_t ws, uintptr_t bias,
                    uintptr_t y, int64_t ldy, int M, int N, int K, int act, bool glu, uintptr_t work, int64_t wbytes,

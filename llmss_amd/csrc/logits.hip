@@ -1,0 +1,274 @@
+// Rules on the logits in front of the sampler: penalties for tokens that were there before, biases of single tokens, and the mask
+// of a grammar's state.
+//
+//   seen(t) = t among the row's known tokens, c(t) = how often among those behind the prompt
+//   y = x;  seen: y = y > 0 ? y / r : y r;   y -= c f;   c > 0: y -= p;   y += the biases of t, in their order;   not allowed: -inf
+//
+// Bound by memory: each logit is read and written once. A workgroup owns a run of CH tokens of a row; it walks the row's known tokens and
+// biases (from the caches: they are few beside the logits) and keeps what concerns its run in LDS - a counter a token, of 16 bits (two
+// in a word) up to 16383 known tokens and 32 beyond, with a bit for "seen" and one for "has a bias"; biases in a hash table. Then it
+// streams its run with 16-byte accesses, and only tokens whose counter is not zero cost more than a copy. Integer counts, and biases
+// summed in the order of the list: the result does not depend on the order in which threads run.
+#include "common.h"
+
+#include <type_traits>
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMostBiases = 1024;
+
+struct LogitRules {
+  const void* x;
+  int64_t ldx;
+  void* y;
+  int64_t ldy;
+  const void* ids;
+  int64_t ldi;
+  int most;  // columns of ids
+  const int *lens, *prompts;
+  const float *rep, *pres, *freq;
+  const int* bias_ids;
+  const float* bias;
+  int64_t ldb;
+  int biases;
+  const unsigned* mask;
+  int64_t ldm;
+  const int* mask_rows;
+  int masks, V, table, wide;  // wide: ids of 64 bits
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const u16x8 x = *reinterpret_cast<const u16x8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = bf2f(x[i]);
+  } else {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = a[i];
+      v[4 + i] = b[i];
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    u16x8 x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = f2bf(v[i]);
+    *reinterpret_cast<u16x8*>(p) = x;
+  } else {
+    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  }
+}
+template <typename T>
+__device__ __forceinline__ float load1(const T* p) {
+  if constexpr (sizeof(T) == 2) return bf2f(*p);
+  else return *p;
+}
+template <typename T>
+__device__ __forceinline__ void store1(T* p, float v) {
+  if constexpr (sizeof(T) == 2) *p = f2bf(v);
+  else *p = v;
+}
+
+__device__ __forceinline__ unsigned hash_of(int t) { return (unsigned)t * 2654435761u; }
+
+// W: 16-bit counters, else 32. VEC: rows of both sides on 16 bytes.
+template <typename TI, typename TO, bool W16, bool VEC>
+__global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRules a, int CH) {
+  extern __shared__ __attribute__((aligned(16))) unsigned lds[];
+  const int b = blockIdx.y, lo = blockIdx.x * CH, n = min(CH, a.V - lo);
+  constexpr unsigned kSeen = W16 ? 0x8000u : 0x80000000u, kBias = W16 ? 0x4000u : 0x40000000u, kCount = kBias - 1;
+  unsigned* cnt = lds;
+  const int words = W16 ? CH / 2 : CH;
+  int* key = (int*)(lds + words);  // hash table of biased tokens: token, first entry, sum
+  int* first = key + a.table;
+  float* sum = (float*)(first + a.table);
+  __shared__ int twice;
+  const TI* x = (const TI*)a.x + (int64_t)b * a.ldx + lo;
+  TO* y = (TO*)a.y + (int64_t)b * a.ldy + lo;
+
+  const float r = a.rep ? a.rep[b] : 1.f, p = a.pres ? a.pres[b] : 0.f, f = a.freq ? a.freq[b] : 0.f;
+  const int len = a.lens && (a.rep || a.pres || a.freq) ? min(max(a.lens[b], 0), a.most) : 0;
+  const int mrow = a.mask ? (a.mask_rows ? a.mask_rows[b] : b) : -1;
+  const unsigned* mask = mrow >= 0 && mrow < a.masks ? a.mask + (int64_t)mrow * a.ldm : nullptr;
+  const bool marks = len > 0 || a.biases > 0;
+  auto mark = [&](int t, unsigned v, bool add) {
+    unsigned* c = W16 ? cnt + (t >> 1) : cnt + t;
+    if (W16 && (t & 1)) v <<= 16;
+    if (add) atomicAdd(c, v);
+    else atomicOr(c, v);
+  };
+  if (marks) {
+    for (int i = threadIdx.x * 4; i < words; i += kThreads * 4) *reinterpret_cast<u32x4*>(cnt + i) = u32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < a.table; i += kThreads) {
+      key[i] = -1;
+      first[i] = INT_MAX;
+    }
+    if (threadIdx.x == 0) twice = 0;
+    __syncthreads();
+    const int prompt = a.prompts ? min(max(a.prompts[b], 0), len) : 0;
+    for (int i = threadIdx.x; i < len; i += kThreads) {
+      const int64_t t = (a.wide ? ((const int64_t*)a.ids)[b * a.ldi + i] : (int64_t)((const int*)a.ids)[b * a.ldi + i]) - lo;
+      if (t < 0 || t >= n) continue;
+      if (i >= prompt) mark((int)t, 1u, true);
+      else mark((int)t, kSeen, false);
+    }
+    // each biased token of the run gets a place in the table; the first of its entries owns it
+    const int* bi = a.bias_ids + (int64_t)b * a.ldb;
+    const float* bv = a.bias + (int64_t)b * a.ldb;
+    auto place = [&](int t) {
+      unsigned h = hash_of(t) & (a.table - 1);
+      while (true) {
+        const int was = atomicCAS(key + h, -1, t);
+        if (was == -1 || was == t) return h;
+        h = (h + 1) & (a.table - 1);
+      }
+    };
+    for (int i = threadIdx.x; i < a.biases; i += kThreads) {
+      const int t = bi[i] - lo;
+      if (bi[i] < 0 || t < 0 || t >= n) continue;
+      if (atomicMin(first + place(t), i) != INT_MAX) twice = 1;
+      mark(t, kBias, false);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.biases; i += kThreads) {
+      const int t = bi[i] - lo;
+      if (bi[i] < 0 || t < 0 || t >= n) continue;
+      const unsigned h = place(t);
+      if (first[h] != i) continue;
+      float s = bv[i];
+      if (twice)
+        for (int j = i + 1; j < a.biases; ++j)
+          if (bi[j] == bi[i]) s += bv[j];
+      sum[h] = s;
+    }
+    __syncthreads();
+  }
+  auto bias_of = [&](int t) {
+    unsigned h = hash_of(t) & (a.table - 1);
+    while (key[h] != t) h = (h + 1) & (a.table - 1);
+    return sum[h];
+  };
+  auto rules = [&](float v, unsigned c, int t) {
+    const unsigned times = c & kCount;
+    if (times || (c & kSeen)) v = v > 0.f ? v / r : v * r;
+    if (times) v = __fsub_rn(__fsub_rn(v, __fmul_rn((float)times, f)), p);
+    if (c & kBias) v += bias_of(t);
+    return v;
+  };
+  auto one = [&](int t) {
+    float v = load1(x + t);
+    if (marks) {
+      const unsigned c = W16 ? (cnt[t >> 1] >> (t & 1 ? 16 : 0)) & 0xffffu : cnt[t];
+      if (c) v = rules(v, c, t);
+    }
+    if (mask && !(mask[(lo + t) >> 5] >> ((lo + t) & 31) & 1)) v = -INFINITY;
+    store1(y + t, v);
+  };
+  if constexpr (!VEC) {
+    for (int t = threadIdx.x; t < n; t += kThreads) one(t);
+  } else {
+    const int n8 = n & ~7;
+    for (int t = threadIdx.x * 8; t < n8; t += kThreads * 8) {
+      float v[8];
+      load8(x + t, v);
+      unsigned open = 0xff;
+      if (mask) open = mask[(lo + t) >> 5] >> ((lo + t) & 31);
+      if (marks) {
+        unsigned c[8], any = 0;
+        if constexpr (W16) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(cnt + t / 2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            c[2 * i] = w[i] & 0xffffu;
+            c[2 * i + 1] = w[i] >> 16;
+            any |= w[i];
+          }
+        } else {
+          const u32x4 w0 = *reinterpret_cast<const u32x4*>(cnt + t), w1 = *reinterpret_cast<const u32x4*>(cnt + t + 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            c[i] = w0[i];
+            c[4 + i] = w1[i];
+            any |= w0[i] | w1[i];
+          }
+        }
+        if (any) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c[i]) v[i] = rules(v[i], c[i], t + i);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = open >> i & 1 ? v[i] : -INFINITY;
+      store8(y + t, v);
+    }
+    for (int t = n8 + threadIdx.x; t < n; t += kThreads) one(t);
+  }
+}
+
+template <typename TI, typename TO>
+void launch_rules(const LogitRules& a, int B, bool w16, hipStream_t st) {
+  const bool vec = ((uintptr_t)a.x | (uintptr_t)a.y) % 16 == 0 && a.ldx * sizeof(TI) % 16 == 0 && a.ldy * sizeof(TO) % 16 == 0;
+  int CH = 1024;
+  while (CH < (w16 ? 16384 : 8192) && (int64_t)B * ((a.V + CH - 1) / CH) > 1024) CH *= 2;
+  const dim3 grid((a.V + CH - 1) / CH, B);
+  const size_t lds = (size_t)(w16 ? CH * 2 : CH * 4) + (size_t)a.table * 12;
+#define LR(W_, V_) adjust_logits_kernel<TI, TO, W_, V_><<<grid, kThreads, lds, st>>>(a, CH)
+  if (w16) {
+    if (vec) LR(true, true);
+    else LR(true, false);
+  } else {
+    if (vec) LR(false, true);
+    else LR(false, false);
+  }
+#undef LR
+}
+
+}  // namespace
+
+void launch_adjust_logits(const void* x, int64_t ldx, bool x32, void* y, int64_t ldy, bool y32, int B, int V, const void* ids, int64_t ldi,
+                          int most, bool ids64, const void* lens, const void* prompts, const void* rep, const void* pres,
+                          const void* freq, const void* bias_ids, const void* bias, int64_t ldb, int biases, const void* mask,
+                          int64_t ldm, const void* mask_rows, int masks, hipStream_t st) {
+  if (B == 0 || V == 0) return;
+  if (B > 65535) throw std::runtime_error("adjust_logits: at most 65535 rows");
+  if (biases > kMostBiases) throw std::runtime_error("adjust_logits: at most 1024 biases a row");
+  LogitRules a;
+  a.x = x;
+  a.ldx = ldx;
+  a.y = y;
+  a.ldy = ldy;
+  a.ids = ids;
+  a.ldi = ldi;
+  a.most = most;
+  a.lens = (const int*)lens;
+  a.prompts = (const int*)prompts;
+  a.rep = (const float*)rep;
+  a.pres = (const float*)pres;
+  a.freq = (const float*)freq;
+  a.bias_ids = (const int*)bias_ids;
+  a.bias = (const float*)bias;
+  a.ldb = ldb;
+  a.biases = bias_ids ? biases : 0;
+  a.mask = (const unsigned*)mask;
+  a.ldm = ldm;
+  a.mask_rows = (const int*)mask_rows;
+  a.masks = masks;
+  a.V = V;
+  a.wide = ids64;
+  a.table = 0;
+  if (a.biases)  // a power of two, at most half full
+    for (a.table = 4; a.table < 2 * a.biases;) a.table *= 2;
+  const bool w16 = most < 0x4000;
+  if (x32) launch_rules<float, float>(a, B, w16, st);
+  else if (y32) launch_rules<bf16_t, float>(a, B, w16, st);
+  else launch_rules<bf16_t, bf16_t>(a, B, w16, st);
+  HIP_CHECK_LAUNCH();
+}

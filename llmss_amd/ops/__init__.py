@@ -216,3 +216,8 @@ head_prep_cache = _route("head_prep_cache")
 window_attn = _route("window_attn")
 window_q_dtype = _route("window_q_dtype")
 mlstm_mix = _route("mlstm_mix")
+
+# ------------------------------------------------------- many completions of one prompt: attention, rules on logits, log-probabilities
+attn_shared = _route("attn_shared")
+adjust_logits = _route("adjust_logits")
+token_logprobs = _route("token_logprobs")

@@ -234,6 +234,211 @@ def attn_extend(q: torch.Tensor, k_cache, v_cache, block_tables, cu_q, ctx_lens,
     return out
 
 
+def _need(cond: bool, msg: str):
+    if not cond:
+        raise ValueError(msg)
+
+
+def attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx_lens, nh, nkv, D, cu_q, max_qlen, max_own, out):
+    """What attn_shared asks of its arguments, on either device: (sequences, fp8 rows, positions that ``max_own`` stands for)."""
+    _need(nkv > 0 and nh > 0 and nh % nkv == 0, "nh must be a multiple of nkv")
+    _need(D in (64, 128, 256), "shared-prefix attention supports head_dim 64/128/256")
+    _need(q.dim() == 2 and q.dtype == torch.bfloat16 and q.stride(1) == 1 and q.shape[1] >= nh * D, "q bf16 [T, >= nh * D]")
+    kv8 = k_cache.dtype == torch.uint8
+    _need(k_cache.dtype in (torch.bfloat16, torch.uint8) and k_cache.dim() == 4 and k_cache.shape[1] == nkv
+          and k_cache.shape[3] == (D + KV8_TAIL if kv8 else D) and k_cache.is_contiguous(),
+          "k_cache bf16 [nb, nkv, bs, D] or uint8 (fp8 rows) [nb, nkv, bs, D + 16]")
+    _need(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype and v_cache.is_contiguous(), "v_cache like k_cache")
+    bs = k_cache.shape[2]
+    _need(k_cache.shape[0] > 0 and bs > 0, "an empty cache")
+    for t, n, nm in ((prefix_table, 1, "prefix_table"), (block_tables, 2, "block_tables"), (ctx_lens, 1, "ctx_lens")):
+        _need(t.dtype == torch.int32 and t.dim() == n and (t.numel() == 0 or t.stride(-1) == 1), f"{nm} must be int32, {n}-D, dense rows")
+    _need(0 <= prefix_len <= prefix_table.numel() * bs, "prefix_len must be between 0 and what prefix_table holds")
+    T = q.shape[0]
+    if cu_q is None:
+        B = T
+        _need(max_qlen == 1, "several tokens a sequence need cu_q")
+    else:
+        _need(cu_q.dtype == torch.int32 and cu_q.dim() == 1 and cu_q.numel() >= 1 and cu_q.is_contiguous(), "cu_q int32 [B + 1]")
+        B = cu_q.numel() - 1
+        _need(max_qlen >= 1, "max_qlen")
+    _need(ctx_lens.numel() >= B and block_tables.shape[0] >= B, "ctx_lens and block_tables need a row for each sequence")
+    room = block_tables.shape[1] * bs
+    if max_own is None:
+        max_own = room
+    _need(0 <= max_own <= room, "max_own must be between 0 and what a row of block_tables holds")
+    if out is not None:
+        _need(out.dtype == torch.bfloat16 and out.dim() == 2 and out.shape[0] >= T and out.shape[1] >= nh * D and out.stride(1) == 1,
+              "out bf16 [>= T, >= nh * D]")
+    return B, kv8, max_own
+
+
+def attn_shared(q: torch.Tensor, k_cache, v_cache, prefix_table, prefix_len: int, block_tables, ctx_lens, nh: int, nkv: int, D: int,
+                scale: float, cu_q=None, max_qlen: int = 1, max_own=None, out=None) -> torch.Tensor:
+    """Attention of a batch whose sequences share their first ``prefix_len`` positions: those lie in the pages of ``prefix_table``
+    [pages] (the last one may be partly used) and are read once for all; position ``prefix_len + i`` of sequence b is position i of
+    the pages of ``block_tables[b]``. ``ctx_lens`` [B] counts a sequence's whole context, prefix and new tokens included. Without
+    ``cu_q`` row b of ``q`` is the last position of sequence b; with it rows cu_q[b] .. cu_q[b + 1] - 1 are its last positions and each
+    sees what is at or before its own. A row whose context is empty gives zeros, rows of no sequence (behind cu_q's last) stay as they
+    are in ``out`` and are not defined without it. ``max_qlen`` and ``max_own`` say how long the longest portion and own part are
+    expected to be: they size the work's cuts, longer ones are right all the same."""
+    B, _, _ = attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx_lens, nh, nkv, D, cu_q, max_qlen,
+                                max_own, out)
+    _need(scale > 0, "scale must be positive")
+    T, g, bs = q.shape[0], nh // nkv, k_cache.shape[2]
+    if out is None:
+        out = torch.zeros(T, nh * D, dtype=q.dtype, device=q.device)
+    cu = [int(c) for c in cu_q.tolist()] if cu_q is not None else list(range(T + 1))
+    for b in range(B):
+        a, e = cu[b], cu[b + 1]
+        ctx = min(int(ctx_lens[b]), prefix_len + block_tables.shape[1] * bs)
+        first = int(ctx_lens[b]) - (e - a)
+        if e == a:
+            continue
+        if ctx <= 0:
+            out[a:e, : nh * D] = 0
+            continue
+        k, v = [], []
+        n = min(ctx, prefix_len)
+        for cache, to in ((k_cache, k), (v_cache, v)):
+            to.append(gather_kv(cache, prefix_table, n).float())
+            if ctx > n:
+                to.append(gather_kv(cache, block_tables[b], ctx - n).float())
+        k, v = (torch.cat(x, 1).repeat_interleave(g, 0) for x in (k, v))
+        qq = q[a:e, : nh * D].view(e - a, nh, D).float().transpose(0, 1)
+        for i in range(e - a):  # (row by row: what a row does not see is not touched, whatever lies there)
+            m = min(max(first + i + 1, 0), ctx)
+            if m == 0:
+                out[a + i, : nh * D] = 0
+                continue
+            w = torch.softmax(torch.matmul(k[:, :m], qq[:, i, :, None]).squeeze(-1) * scale, -1)
+            out[a + i, : nh * D] = torch.matmul(w[:, None], v[:, :m]).reshape(-1).to(q.dtype)
+    return out
+
+
+def adjust_logits_check(logits, ids, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, mask, mask_rows, vocab, out):
+    """What adjust_logits asks of its arguments, on either device: (rows, vocabulary)."""
+    _need(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and (logits.shape[1] <= 1 or logits.stride(1) == 1),
+          "logits bf16 / fp32 [B, >= vocab], dense rows")
+    B = logits.shape[0]
+    V = logits.shape[1] if vocab is None else int(vocab)
+    _need(0 < V <= logits.shape[1], "vocab must be between 1 and the width of logits")
+    penalties = repetition is not None or presence is not None or frequency is not None
+    _need((ids is None) == (lens is None), "ids and lens go together")
+    _need(not penalties or ids is not None, "penalties need ids and lens")
+    if ids is not None:
+        _need(ids.dtype in (torch.int64, torch.int32) and ids.dim() == 2 and ids.shape[0] >= B
+              and (ids.shape[1] <= 1 or ids.stride(1) == 1), "ids int64 / int32 [B, known tokens], dense rows")
+        _need(lens.dtype == torch.int32 and lens.dim() == 1 and lens.numel() >= B and lens.is_contiguous(), "lens int32 [B]")
+        _need(ids.shape[1] < 1 << 30, "too many known tokens")
+    if prompt_lens is not None:
+        _need(prompt_lens.dtype == torch.int32 and prompt_lens.dim() == 1 and prompt_lens.numel() >= B and prompt_lens.is_contiguous(),
+              "prompt_lens int32 [B]")
+    for t, nm in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
+        _need(t is None or (t.dtype == torch.float32 and t.dim() == 1 and t.numel() >= B and t.is_contiguous()), f"{nm} float32 [B]")
+    _need((bias is None) == (bias_ids is None), "bias and bias_ids go together")
+    if bias is not None:
+        _need(bias_ids.dtype == torch.int32 and bias_ids.dim() == 2 and bias_ids.shape[0] >= B and bias_ids.is_contiguous(),
+              "bias_ids int32 [B, biases]")
+        _need(bias.dtype == torch.float32 and bias.shape == bias_ids.shape and bias.is_contiguous(), "bias float32 like bias_ids")
+        _need(bias_ids.shape[1] <= 1024, "at most 1024 biases a row")
+    _need(mask is not None or mask_rows is None, "mask_rows without a mask")
+    if mask is not None:
+        _need(mask.dtype == torch.int32 and mask.dim() == 2 and mask.shape[1] * 32 >= V and (mask.shape[1] <= 1 or mask.stride(1) == 1),
+              "mask int32 [masks, >= vocab / 32], dense rows")
+        _need(mask_rows is not None or mask.shape[0] >= B, "a mask row for each row, or mask_rows")
+        if mask_rows is not None:
+            _need(mask_rows.dtype == torch.int32 and mask_rows.dim() == 1 and mask_rows.numel() >= B and mask_rows.is_contiguous(),
+                  "mask_rows int32 [B]")
+    if out is not None:
+        _need(out.dim() == 2 and out.shape[0] >= B and out.shape[1] >= V and (out.shape[1] <= 1 or out.stride(1) == 1)
+              and out.dtype in (logits.dtype, torch.float32), "out [B, >= vocab] in the type of logits or fp32, dense rows")
+    return B, V
+
+
+def adjust_logits(logits: torch.Tensor, ids=None, lens=None, prompt_lens=None, repetition=None, presence=None, frequency=None,
+                  bias_ids=None, bias=None, mask=None, mask_rows=None, vocab=None, out=None) -> torch.Tensor:
+    """The rules in front of the sampler, on rows of logits [B, >= vocab]; returns [B, vocab] in their type, or ``out`` (which may be
+    ``logits`` itself, or fp32). ``ids`` [B, n] are the row's known tokens, ``lens`` [B] how many, ``prompt_lens`` [B] how many of them
+    are its prompt (none without it). A token that is known has its logit divided by ``repetition`` where positive and multiplied where
+    not; one that came c > 0 times behind the prompt loses ``c * frequency + presence``; entries (``bias_ids``, ``bias``) [B, m] are added
+    in their order (a negative id is no entry); tokens whose bit in the row's mask is clear get -inf: bit t % 32 of word t // 32 of
+    ``mask[mask_rows[b]]`` (``mask[b]`` without mask_rows; a mask row that does not exist, as -1, allows every token). Ids outside the
+    vocabulary are passed over."""
+    B, V = adjust_logits_check(logits, ids, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, mask, mask_rows, vocab, out)
+    x = logits[:, :V]
+    y = x.float().clone()
+    if repetition is not None or presence is not None or frequency is not None:
+        for b in range(B):
+            n = min(max(int(lens[b]), 0), ids.shape[1])
+            p = min(max(int(prompt_lens[b]), 0), n) if prompt_lens is not None else 0
+            known = ids[b, :n].long()
+            ok = (known >= 0) & (known < V)
+            every = torch.unique(known[ok])
+            said, times = torch.unique(known[p:][ok[p:]], return_counts=True)
+            row = y[b]
+            if repetition is not None:
+                row[every] = torch.where(row[every] > 0, row[every] / repetition[b], row[every] * repetition[b])
+            if frequency is not None:
+                row[said] -= times.float() * frequency[b]
+            if presence is not None:
+                row[said] -= presence[b]
+    if bias is not None:
+        for b in range(B):
+            add = {}
+            for t, v in zip(bias_ids[b].tolist(), bias[b].tolist()):
+                if 0 <= t < V:
+                    add[t] = float(np.float32(add[t]) + np.float32(v)) if t in add else v
+            for t, v in add.items():
+                y[b, t] += v
+    if mask is not None:
+        t = torch.arange(V, device=mask.device)
+        for b in range(B):
+            r = int(mask_rows[b]) if mask_rows is not None else b
+            if 0 <= r < mask.shape[0]:
+                y[b, ((mask[r].long()[t >> 5] >> (t & 31)) & 1) == 0] = float("-inf")
+    if out is None:
+        return y.to(logits.dtype)
+    out[:B, :V] = y.to(out.dtype)
+    return out[:B, :V]
+
+
+def token_logprobs_check(logits, tokens, top_n, vocab):
+    """What token_logprobs asks of its arguments, on either device: (rows, vocabulary)."""
+    _need(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and (logits.shape[1] <= 1 or logits.stride(1) == 1),
+          "logits bf16 / fp32 [B, >= vocab], dense rows")
+    B = logits.shape[0]
+    V = logits.shape[1] if vocab is None else int(vocab)
+    _need(0 < V <= logits.shape[1], "vocab must be between 1 and the width of logits")
+    _need(tokens is None or (tokens.dtype == torch.int64 and tokens.dim() == 1 and tokens.numel() >= B and tokens.is_contiguous()),
+          "tokens int64 [B]")
+    _need(0 <= top_n <= min(64, V), "top_n must be between 0 and min(64, vocab)")
+    return B, V
+
+
+def token_logprobs(logits: torch.Tensor, tokens, top_n: int = 0, vocab=None):
+    """(log-probability [B] fp32 and rank [B] int64 of ``tokens`` [B] under rows of logits; ids [B, top_n] int64 and log-probabilities
+    [B, top_n] fp32 of the likeliest tokens, equal logits by falling id last). A rank is 1 for the likeliest: 1 + how many logits are
+    greater. A token outside the vocabulary (-1: none) has log-probability and rank 0. Over a row of nothing but -inf every token's is
+    -inf; a NaN among the logits makes the row's log-probabilities NaN and is not among the likeliest (places that are left over hold id -1)."""
+    B, V = token_logprobs_check(logits, tokens, top_n, vocab)
+    x = logits[:, :V].float()
+    lp = torch.log_softmax(x.double(), -1)
+    lp = torch.where((x == float("-inf")).all(-1, keepdim=True), torch.full_like(lp, float("-inf")), lp).float()
+    tok = tokens[:B] if tokens is not None else torch.full((B,), -1, dtype=torch.int64, device=x.device)
+    given = (tok >= 0) & (tok < V)
+    at = tok.clamp(0, V - 1)[:, None]
+    mine = torch.where(given, lp.gather(1, at)[:, 0], torch.zeros(B, device=x.device))
+    rank = torch.where(given, 1 + (x > x.gather(1, at)).sum(-1), torch.zeros_like(tok))
+    order = torch.sort(torch.where(x.isnan(), torch.full_like(x, float("-inf")), x), dim=-1, descending=True, stable=True)[1]
+    # (a NaN stands behind every number, -inf too)
+    order = torch.stack([torch.cat([o[~n[o]], o[n[o]]]) for o, n in zip(order, x.isnan())]) if B else order
+    ids = order[:, :top_n]
+    ids = torch.where(x.isnan().gather(1, ids), torch.full_like(ids, -1), ids)
+    top = lp.gather(1, ids.clamp(min=0))
+    return mine, rank, ids, torch.where(ids < 0, torch.full_like(top, float("nan")), top)
+
+
 def glu_split(w_or_y: torch.Tensor, dim: int = -1):
     """Split a 16-row/column interleaved gate|up tensor into (gate, up)."""
     n = w_or_y.shape[dim]
