@@ -44,7 +44,11 @@ struct SharedAttn {
   const int* cu;   // null: row t is sequence t
   const int* ctx;  // positions of a sequence's context, its new ones among them
   float *po, *pml;
-  int T, B, nh, nkv, G, bs, shift, pages, P, own_cap;  // shift: log2 of bs where it is a power of two, or -1
+  bf16_t* out;
+  int64_t out_stride;
+  int parts, finish;  // partial results of a (row, head); whether the own parts' launch joins them itself
+  int64_t page_bytes;
+  int T, B, nh, nkv, G, bs, shift, pages, P, own_cap;  // shift: log2 of bs where it is a power of two
   int pre_items, pre_tiles, pre_split, pre_keys, pre_few;
   int own_tiles, own_split, own_keys, own_few;
   float scale_log2;
@@ -81,28 +85,55 @@ __device__ __forceinline__ int slot_limit(const SharedAttn& a, const Item& it, i
   return it.own ? min(max(n - a.P, 0), a.own_cap) : min(n, a.P);
 }
 
-// The cache row of a key: pages of 16 m positions are asked once for 16 keys, by a scalar load.
-template <bool BY16>
+// Where the cache rows of a tile of 16 KT keys lie, in bytes. Pages of 16, 32, 64 .. positions (BY16): a lane asks for the page of one
+// run of 16 keys, a tile ahead (a vector load, which the wait in front of the next tile covers: a scalar one would have the reads of
+// LDS wait for it); a run's address is formed in scalar registers, a lane adds 32 bits. Others: each row asks for its own page where
+// it is needed. RB: bytes of a cache row.
+template <bool BY16, int KT, int RB>
 struct Rows {
   const SharedAttn& a;
   const Item& it;
-  int64_t row_size;  // of one cache row, in cache elements
-  __device__ __forceinline__ int64_t in_page(int k) const {
-    const int i = a.shift >= 0 ? k >> a.shift : k / a.bs;
-    const unsigned p = (unsigned)it.table[i];
-    return (((int64_t)(p < (unsigned)a.pages ? p : 0) * a.nkv + it.kvh) * a.bs + (k - i * a.bs)) * row_size;
+  int ids = 0;
+  __device__ __forceinline__ int64_t start(int page) const {
+    const unsigned p = (unsigned)page < (unsigned)a.pages ? (unsigned)page : 0u;
+    return (int64_t)p * a.page_bytes + (int64_t)it.kvh * a.bs * RB;
   }
-  // key k16 + r, at most the last one; k16 the same in every lane and a multiple of 16, r < 16
-  __device__ __forceinline__ int64_t at(int k16, int r) const {
-    const int last = it.stop - 1;
+  __device__ __forceinline__ void ask(int kv0) {  // (in front of other accesses to memory: else it is moved to where its answer is used)
+    if constexpr (BY16) ids = it.table[min(kv0 + 16 * (int)(threadIdx.x % KT), it.stop - 1) >> a.shift];
+  }
+  __device__ __forceinline__ int page(int run) const { return BY16 ? __builtin_amdgcn_readlane(ids, run) : 0; }
+  // row r < 16 of run `run` of a tile, whose page is pg (both the same in every lane); keys past the last stand for the last
+  __device__ __forceinline__ int base(int kv0, int run) const { return min(kv0 + 16 * run, (it.stop - 1) & ~15); }
+  __device__ __forceinline__ int64_t run_at(int pg, int kv0, int run) const { return start(pg) + (base(kv0, run) & (a.bs - 1)) * RB; }
+  __device__ __forceinline__ unsigned row_at(int kv0, int run, int r) const { return min(r, it.stop - 1 - base(kv0, run)) * RB; }
+  __device__ __forceinline__ int64_t alone(int k) const {
+    k = min(k, it.stop - 1);
+    const int i = k / a.bs;
+    return start(it.table[i]) + (k - i * a.bs) * RB;
+  }
+  template <typename V>
+  __device__ __forceinline__ V load(const void* cache, int pg, int kv0, int run, int r, unsigned more) const {
+    if constexpr (BY16) return *reinterpret_cast<const V*>((const char*)cache + run_at(pg, kv0, run) + (row_at(kv0, run, r) + more));
+    else return *reinterpret_cast<const V*>((const char*)cache + alone(kv0 + 16 * run + r) + more);
+  }
+  // 16 bytes a lane from memory into LDS (lane l at lds + 16 l). Through inline assembly, so that the compiler does not hold reads
+  // of other places in LDS back until it has landed: every use stands behind a wait for vmcnt(0) of its own.
+  __device__ __forceinline__ void to_lds(const void* cache, int pg, int kv0, int run, int r, unsigned more, char* lds) const {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LDS_AS char*)lds);
     if constexpr (BY16) {
-      const int base = __builtin_amdgcn_readfirstlane(min(k16, last & ~15));
-      return in_page(base) + min(r, last - base) * row_size;
+      const char* p = (const char*)cache + run_at(pg, kv0, run);
+      const unsigned off = row_at(kv0, run, r) + more;
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory");
     } else {
-      return in_page(min(k16 + r, last));
+      const char* p = (const char*)cache + alone(kv0 + 16 * run + r) + more;
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory");
     }
   }
 };
+
+// Has the compiler wait for what was loaded into x: a first use inside a loop would be waited for in every turn, and with it
+// for the loads into LDS that it does not count.
+__device__ __forceinline__ void landed(s16x8& x) { asm volatile("" : "+v"(x)); }
 
 __device__ __forceinline__ s16x8 fp8_to_bf16(unsigned lo, unsigned hi) {
   const u32x4 o = {__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
@@ -207,10 +238,12 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS],
 // O^T += V^T P^T. Where a tile that is masked for some slots holds values that are not finite, the products would give them to every
 // slot (0 times such a value is NaN): there the weights go through `own_lds` (16 slots of 16 KT keys, the wave's own) and each slot
 // takes the keys that it sees one after the other. Rare, so kept small.
-template <int D, int KT, int NS, bool MASK>
-__device__ __forceinline__ void add_values(const char* img, bf16_t* own_lds, const int (&lim)[NS], int g, int li,
+template <int D, int KT, int NS>
+__device__ __forceinline__ void add_values(bool masked, const char* img, bf16_t* own_lds, const int (&lim)[NS], int g_, int li_,
                                            const s16x8 (&pf)[NS][KT / 2], f32x4 (&o)[NS][D / 16]) {
-  if constexpr (MASK) {
+  if (masked) {
+    int g = g_, li = li_;
+    asm volatile("" : "+v"(g), "+v"(li));  // (the rare path's addresses are formed in it and hold no registers outside)
     unsigned bad = 0;
 #pragma unroll
     for (int k = 0; k < KT / 2; ++k)
@@ -251,15 +284,54 @@ __device__ __forceinline__ void add_values(const char* img, bf16_t* own_lds, con
   for (int k = 0; k < KT / 2; ++k)
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
-      const s16x8 vf = v_fragment<D>(img, 32 * k, dt, g, li);
+      const s16x8 vf = v_fragment<D>(img, 32 * k, dt, g_, li_);
 #pragma unroll
       for (int n = 0; n < NS; ++n) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][k], o[n][dt], 0, 0, 0);
+      if (KT == 2 && NS == 1 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (second form: no registers for more reads ahead)
     }
 }
 
+// A softmax over several sets of keys from the sets' (m, l) and four of their outputs.
+struct Joined {
+  float top = kFloor, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(f32x2 ml, f32x4 x) {
+    if (ml[1] == 0.f) return;  // (a set without a visible key; its outputs may be anything)
+    const float t = fmaxf(top, ml[0]), f = __builtin_amdgcn_exp2f(top - t), h = __builtin_amdgcn_exp2f(ml[0] - t);
+    top = t;
+    l = l * f + ml[1] * h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * f + x[e] * h;
+  }
+  // parts that lie one after the other, eight asked for at a time
+  template <int D>
+  __device__ __forceinline__ void add_parts(const float* ml, const float* x, int n) {
+    for (int p = 0; p < n; p += 8) {
+      f32x2 b[8];
+      f32x4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int q = min(p + i, n - 1);
+        b[i] = *reinterpret_cast<const f32x2*>(ml + 2 * q);
+        v[i] = *reinterpret_cast<const f32x4*>(x + (int64_t)q * D);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (p + i < n) add(b[i], v[i]);
+    }
+  }
+  __device__ __forceinline__ void store(bf16_t* out) const {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    u16x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = f2bf(o[e] * inv);
+    *reinterpret_cast<u16x4*>(out) = r;
+  }
+};
+
 template <int D>
 __device__ __forceinline__ void leave(const SharedAttn& a, const Item& it, int slot, int g, const f32x4 (&o)[D / 16], float m, float l) {
-  const int64_t pi = ((int64_t)(it.row0 + slot / a.G) * a.nh + it.kvh * a.G + slot % a.G) * (a.pre_split + a.own_split) + it.part;
+  const int64_t pi = ((int64_t)(it.row0 + slot / a.G) * a.nh + it.kvh * a.G + slot % a.G) * a.parts + it.part;
 #pragma unroll
   for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(a.po + pi * D + dt * 16 + 4 * g) = o[dt];
   if (g == 0) {
@@ -295,7 +367,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
   __syncthreads();  // (a workgroup may have had an item before)
   if (lane == 0) red[w] = wave_hi;
   __syncthreads();
-  it.stop = min(it.stop, max(max(red[0], red[1]), max(red[2], red[3])));
+  it.stop = __builtin_amdgcn_readfirstlane(min(it.stop, max(max(red[0], red[1]), max(red[2], red[3]))));
 
   f32x4 o[NS][D / 16], lsum[NS];
   float m[NS];
@@ -315,7 +387,11 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
 #pragma unroll
       for (int ks = 0; ks < D / 32; ++ks) qf[n][ks] = *reinterpret_cast<const s16x8*>(qp + 32 * ks);
     }
-    const Rows<BY16> rows{a, it, KV8 ? D + kTail : D};
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks) landed(qf[n][ks]);
+    Rows<BY16, KT, KV8 ? D + kTail : 2 * D> rows{a, it};
     const int ntiles = (it.stop - it.begin + BKV - 1) / BKV;
 
     // bf16: 16 bytes a lane straight into LDS, a wave's instruction covers RPI rows
@@ -325,29 +401,34 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
     u32x4 k8[KV8 ? PIECES : 1], v8[KV8 ? PIECES : 1];
     float sc = 0.f;
     auto fetch = [&](int j) {
+      int lane = threadIdx.x & 63;
+      asm volatile("" : "+v"(lane));  // (what follows from it is formed here and holds no registers in between)
       const int kv0 = it.begin + j * BKV;
       char* sk = smem + (j & 1) * 2 * TILE;
       if constexpr (KV8) {
+        int pg[PIECES];
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)  // (16 rows of 4, 8 or 16 pieces: a wave's rows lie within one run of 16)
+          pg[i] = rows.page(__builtin_amdgcn_readfirstlane((threadIdx.x + i * 256) / D));
+        rows.ask(kv0 + BKV);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-          const int c = threadIdx.x + i * 256, r = c / (D / 16);
-          // (16 rows of 4, 8 or 16 pieces: a wave's rows lie within one run of 16)
-          const int64_t off = rows.at(kv0 + __builtin_amdgcn_readfirstlane(r & ~15), r & 15) + (c % (D / 16)) * 16;
-          k8[i] = *reinterpret_cast<const u32x4*>((const unsigned char*)a.kc + off);
-          v8[i] = *reinterpret_cast<const u32x4*>((const unsigned char*)a.vc + off);
+          const int c = threadIdx.x + i * 256, r = c / (D / 16), run = __builtin_amdgcn_readfirstlane(c / D);
+          k8[i] = rows.template load<u32x4>(a.kc, pg[i], kv0, run, r & 15, (c % (D / 16)) * 16);
+          v8[i] = rows.template load<u32x4>(a.vc, pg[i], kv0, run, r & 15, (c % (D / 16)) * 16);
         }
-        if (threadIdx.x < 2 * BKV) {
-          const Rows<false> one{a, it, D + kTail};
-          const int64_t off = one.at(kv0, threadIdx.x % BKV) + D;
-          sc = *reinterpret_cast<const float*>((const unsigned char*)(threadIdx.x < BKV ? a.kc : a.vc) + off);
-        }
+        if (threadIdx.x < 2 * BKV)
+          sc = *reinterpret_cast<const float*>((const char*)(threadIdx.x < BKV ? a.kc : a.vc) + rows.alone(kv0 + threadIdx.x % BKV) + D);
       } else {
+        int pg[LPW];
+#pragma unroll
+        for (int i = 0; i < LPW; ++i) pg[i] = rows.page((i * 4 + w) * RPI / 16);
+        rows.ask(kv0 + BKV);
 #pragma unroll
         for (int i = 0; i < LPW; ++i) {
           const int inst = i * 4 + w, r = inst * RPI + lane / CH;
-          const int64_t off = rows.at(kv0 + (inst * RPI & ~15), r & 15) + swz<D>(lane % CH, r) * 8;
-          __builtin_amdgcn_global_load_lds((const void*)((const bf16_t*)a.kc + off), (LDS_AS void*)(sk + inst * 1024), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds((const void*)((const bf16_t*)a.vc + off), (LDS_AS void*)(sk + TILE + inst * 1024), 16, 0, 0);
+          rows.to_lds(a.kc, pg[i], kv0, inst * RPI / 16, r & 15, swz<D>(lane % CH, r) << 4, sk + inst * 1024);
+          rows.to_lds(a.vc, pg[i], kv0, inst * RPI / 16, r & 15, swz<D>(lane % CH, r) << 4, sk + TILE + inst * 1024);
         }
       }
     };
@@ -406,10 +487,11 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
       for (int n = 0; n < NS; ++n) left[n] = MASK ? min(lim[n], it.stop) - kv0 : BKV;
       s16x8 pf[NS][KT / 2];
       soften<D, KT, NS, MASK>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
-      add_values<D, KT, NS, MASK>(sk + TILE, apart + w * 16 * BKV, left, g, li, pf, o);
+      add_values<D, KT, NS>(MASK, sk + TILE, apart + w * 16 * BKV, left, g, li, pf, o);
     };
     // tiles that every slot of the wave sees whole come first, in a loop without masks
     const int whole = min(max(0, (min(wave_lo, it.stop) - it.begin) / BKV), ntiles);
+    rows.ask(it.begin);
     fetch(0);
     if constexpr (KV8) {
       put(0);
@@ -451,7 +533,6 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
 template <int D, bool KV8, bool BY16>
 __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char* smem, float* scales, bf16_t* apart) {
   constexpr int KT = 2, BK = 32, CH = D / 8;
-  constexpr int PLACES = D == 256 ? 1 : 2;  // of values: wide heads' would take all of LDS
   constexpr int TILE = BK * D * 2;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, g = lane >> 4;
@@ -467,7 +548,9 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) o[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   __syncthreads();  // (a workgroup may have had an item before: the places below are free)
-  if (it.stop > it.begin) {
+  const int step = 4 * BK;
+  int kv0 = it.begin + w * BK;
+  if (kv0 < it.stop) {
     s16x8 qf[D / 32];
     {
       const int sl = min(slot, it.slots - 1);
@@ -476,59 +559,70 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       for (int ks = 0; ks < D / 32; ++ks)
         qf[ks] = *reinterpret_cast<const s16x8*>(qp + (KV8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g));
     }
-    const Rows<BY16> rows{a, it, KV8 ? D + kTail : D};
-    char* const mine = smem + w * PLACES * TILE;
+    Rows<BY16, KT, KV8 ? D + kTail : 2 * D> rows{a, it};
+    char* const img = smem + w * TILE;
     float* const fac = scales + w * 2 * BK;  // (fp8) scales of the keys, of the values
     s16x8 kf[KT][KV8 ? 1 : D / 32];
     u32x4 k8[KT][KV8 ? D / 64 : 1];
     constexpr int RPI = 64 / CH, INS = BK / RPI, PIECES = BK * (D / 16) / 64;
     u32x4 v8[KV8 ? PIECES : 1];
     float sc = 0.f;
-    auto keys = [&](int kv0) {
+    // (a lane's number as something new each time: what follows from it is formed where it is used and holds no registers in between)
+    auto anew = [&]() {
+      int l = lane;
+      asm volatile("" : "+v"(l));
+      return l;
+    };
+    auto keys = [&](int kv0, const int (&pg)[KT]) {
+      const int l = anew(), li = l & 15, g = l >> 4;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        const int64_t off = rows.at(kv0 + kt * 16, li);
         if constexpr (KV8) {
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c) k8[kt][c] = *reinterpret_cast<const u32x4*>((const unsigned char*)a.kc + off + 64 * c + 16 * g);
+          for (int c = 0; c < D / 64; ++c) k8[kt][c] = rows.template load<u32x4>(a.kc, pg[kt], kv0, kt, li, 64 * c + 16 * g);
         } else {
 #pragma unroll
-          for (int ks = 0; ks < D / 32; ++ks) kf[kt][ks] = *reinterpret_cast<const s16x8*>((const bf16_t*)a.kc + off + 32 * ks + 8 * g);
+          for (int ks = 0; ks < D / 32; ++ks) kf[kt][ks] = rows.template load<s16x8>(a.kc, pg[kt], kv0, kt, li, 64 * ks + 16 * g);
         }
       }
-      if constexpr (KV8) {
-        const Rows<false> one{a, it, D + kTail};
-        sc = *reinterpret_cast<const float*>((const unsigned char*)(lane < BK ? a.kc : a.vc) + one.at(kv0, lane % BK) + D);
-      }
+      if constexpr (KV8) sc = *reinterpret_cast<const float*>((const char*)(lane < BK ? a.kc : a.vc) + rows.alone(kv0 + lane % BK) + D);
     };
-    auto values = [&](int kv0, int place) {
+    auto values = [&](int kv0, const int (&pg)[KT]) {
+      const int lane = anew();
       if constexpr (KV8) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int c = lane + i * 64, r = c / (D / 16);
-          const int64_t off = rows.at(kv0 + __builtin_amdgcn_readfirstlane(r & ~15), r & 15) + (c % (D / 16)) * 16;
-          v8[i] = *reinterpret_cast<const u32x4*>((const unsigned char*)a.vc + off);
+          const int run = i * 64 / D;  // (16 rows are D pieces)
+          v8[i] = rows.template load<u32x4>(a.vc, pg[run], kv0, run, r & 15, (c % (D / 16)) * 16);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < INS; ++i) {
           const int r = i * RPI + lane / CH;
-          const int64_t off = rows.at(kv0 + (i * RPI & ~15), r & 15) + swz<D>(lane % CH, r) * 8;
-          __builtin_amdgcn_global_load_lds((const void*)((const bf16_t*)a.vc + off), (LDS_AS void*)(mine + place * TILE + i * 1024), 16, 0, 0);
+          rows.to_lds(a.vc, pg[i * RPI / 16], kv0, i * RPI / 16, r & 15, swz<D>(lane % CH, r) << 4, img + i * 1024);
         }
       }
     };
-    const int step = 4 * BK;
-    int kv0 = it.begin + w * BK, place = 0;
-    if (kv0 < it.stop) {
-      keys(kv0);
-      values(kv0, 0);
-    }
+    int pg[KT];
+    auto pages = [&](int kv0) {  // those asked for, and what lies a turn behind them is asked for
+#pragma unroll
+      for (int i = 0; i < KT; ++i) pg[i] = rows.page(i);
+      rows.ask(kv0 + step);
+    };
+    rows.ask(kv0);
+    pages(kv0);
+    keys(kv0, pg);
+    values(kv0, pg);
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) landed(qf[ks]);
     for (; kv0 < it.stop; kv0 += step) {
       const int nx = kv0 + step;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this run's keys and values
-      char* img = mine + place * TILE;
+      pages(nx);
+      asm volatile("" ::: "memory");
       if constexpr (KV8) {
+        const int lane = anew();
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int c = lane + i * 64, r = c / (D / 16), c0 = (c % (D / 16)) * 2;
@@ -538,8 +632,6 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
         }
         fac[lane] = sc;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      } else if constexpr (PLACES == 2) {
-        if (nx < it.stop) values(nx, place ^ 1);
       }
       f32x4 s[1][KT];
 #pragma unroll
@@ -553,9 +645,10 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
           else f = kf[kt][ks];
           s[0][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[ks], s[0][kt], 0, 0, 0);
         }
-      if (nx < it.stop) {
-        keys(nx);
-        if constexpr (KV8) values(nx, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (nx < it.stop) {  // the next run's keys come while this one's values are used
+        keys(nx, pg);
+        if constexpr (KV8) values(nx, pg);
       }
       if constexpr (KV8) {
 #pragma unroll
@@ -568,17 +661,15 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       const float* vs = KV8 ? fac + BK : nullptr;
       s16x8 pf[1][1];
       const int left[1] = {min(lim[0], it.stop) - kv0};
-      if (kv0 + BK <= min(lo, it.stop)) {
-        soften<D, KT, 1, false>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
-        add_values<D, KT, 1, false>(img, apart + w * 16 * BK, left, g, li, pf, o);
-      } else {
-        soften<D, KT, 1, true>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
-        add_values<D, KT, 1, true>(img, apart + w * 16 * BK, left, g, li, pf, o);
+      soften<D, KT, 1, true>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
+      const int l = anew();
+      add_values<D, KT, 1>(kv0 + BK > min(lo, it.stop), img, apart + w * 16 * BK, left, l >> 4, l & 15, pf, o);
+      if (nx < it.stop) {
+        if constexpr (!KV8) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the place is read)
+          values(nx, pg);
+        }
       }
-      if constexpr (!KV8 && PLACES == 1) {
-        if (nx < it.stop) values(nx, 0);  // (the reads of this run's were waited for by the products)
-      }
-      if constexpr (PLACES == 2) place ^= 1;
     }
   }
   // the waves meet: outputs [wave][slot][D] and (m, l)
@@ -595,53 +686,44 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
   for (int c = threadIdx.x; c < 16 * (D / 4); c += 256) {
     const int sl = c / (D / 4), d4 = c % (D / 4);
     if (it.first + sl >= it.slots) continue;
-    float top = kFloor, l = 0.f;
+    Joined j;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, scales[(i * 16 + sl) * 2]);
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float li_ = scales[(i * 16 + sl) * 2 + 1];
-      if (li_ == 0.f) continue;  // (this wave saw none of its keys)
-      const float f = __builtin_amdgcn_exp2f(scales[(i * 16 + sl) * 2] - top);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(so + (i * 16 + sl) * LDO + d4 * 4);
-      l += li_ * f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += x[e] * f;
-    }
+    for (int i = 0; i < 4; ++i)
+      j.add(*reinterpret_cast<const f32x2*>(scales + (i * 16 + sl) * 2), *reinterpret_cast<const f32x4*>(so + (i * 16 + sl) * LDO + d4 * 4));
     const int s_ = it.first + sl;
-    const int64_t pi = ((int64_t)(it.row0 + s_ / a.G) * a.nh + it.kvh * a.G + s_ % a.G) * (a.pre_split + a.own_split) + it.part;
-    *reinterpret_cast<f32x4*>(a.po + pi * D + d4 * 4) = sum;
-    if (d4 == 0) {
-      a.pml[pi * 2] = top;
-      a.pml[pi * 2 + 1] = l;
+    const int64_t row = it.row0 + s_ / a.G, head = it.kvh * a.G + s_ % a.G;
+    if (it.own && a.finish) {  // the own part is one workgroup's: the prefix's parts, left by the launch before, join it here
+      const int64_t pi = (row * a.nh + head) * a.parts;
+      j.add_parts<D>(a.pml + pi * 2, a.po + pi * D + d4 * 4, a.pre_split);
+      j.store(a.out + row * a.out_stride + head * D + d4 * 4);
+    } else {
+      const int64_t pi = (row * a.nh + head) * a.parts + it.part;
+      *reinterpret_cast<f32x4*>(a.po + pi * D + d4 * 4) = j.o;
+      if (d4 == 0) *reinterpret_cast<f32x2*>(a.pml + pi * 2) = f32x2{j.top, j.l};
     }
   }
 }
 
-// FORMS: which forms the items take, by waves' rows (r) or keys (k): the prefix's and the own parts'.
-enum Forms { RR = 0, RK = 1, KK = 2 };
+enum Form { ROWS, KEYS };
 
-template <int D, bool KV8, int NS, int FORMS, bool BY16>
-__global__ __launch_bounds__(256, 2) void attn_shared_kernel(const SharedAttn a) {
-  constexpr int ROWS = 2 * 2 * tile_keys(D) * D * 2;                      // tiles of the first form
-  constexpr int KEYS = 4 * (D == 256 ? 1 : 2) * 32 * D * 2;                // places of values of the second
-  constexpr int MEET = 4 * 16 * (D + 4) * 4;                               // its outputs
-  constexpr int SECOND = KEYS > MEET ? KEYS : MEET;
-  constexpr int SIZE = FORMS == RR ? ROWS : FORMS == KK ? SECOND : ROWS > SECOND ? ROWS : SECOND;
-  __shared__ __attribute__((aligned(16))) char smem[SIZE];
-  __shared__ __attribute__((aligned(16))) float scales[4 * 2 * 64];
-  __shared__ __attribute__((aligned(16))) bf16_t apart[4 * 16 * (FORMS == KK ? 32 : tile_keys(D))];
+// Items [0, pre_items) are the prefix's, the others own parts. The second form is bound by memory and takes few registers and little LDS:
+// more of its workgroups share a compute unit.
+template <int D, bool KV8, int NS, int FORM, bool BY16>
+__global__ __launch_bounds__(256, FORM == KEYS ? (D == 64 ? 4 : D == 128 ? 3 : 2) : 2) void attn_shared_kernel(const SharedAttn a) {
+  constexpr int PLACES = FORM == ROWS ? 2 * 2 * tile_keys(D) * D * 2 : 4 * 32 * D * 2;  // tiles; each wave's values
+  constexpr int MEET = FORM == ROWS ? 0 : 4 * 16 * (D + 4) * 4;                         // the second form's outputs
+  __shared__ __attribute__((aligned(16))) char smem[PLACES > MEET ? PLACES : MEET];
+  __shared__ __attribute__((aligned(16))) float scales[FORM == ROWS ? (KV8 ? 2 * 2 * tile_keys(D) : 4) : 4 * 2 * 32];
+  __shared__ __attribute__((aligned(16))) bf16_t apart[4 * 16 * (FORM == KEYS ? 32 : tile_keys(D))];
   __shared__ int red[4];
+  constexpr int per = FORM == KEYS ? 16 : 64 * NS;
   Item it;
-  int id = blockIdx.x;
-  int tile, tiles, per;
+  int id = blockIdx.x, tile, tiles;
   if (id < a.pre_items) {  // (key head, run of keys, tile of slots), the tiles of a run on one die
     id = xcd_remap(id, a.pre_items);
     const int run = id / a.pre_tiles;
     tile = id % a.pre_tiles;
-    tiles = INT_MAX / 1024;
-    per = FORMS == KK ? 16 : 64 * NS;
+    tiles = INT_MAX / 1024;  // (one turn)
     it.own = 0;
     it.table = a.prefix_table;
     it.row0 = 0;
@@ -655,7 +737,6 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const SharedAttn a)
     const int run = id % a.own_split;
     tile = id / a.own_split % a.own_tiles;
     tiles = a.own_tiles;
-    per = FORMS == RR ? 64 * NS : 16;
     it.own = 1;
     it.kvh = id / a.own_split / a.own_tiles % a.nkv;
     const int b = id / a.own_split / a.own_tiles / a.nkv;
@@ -669,42 +750,23 @@ __global__ __launch_bounds__(256, 2) void attn_shared_kernel(const SharedAttn a)
   // (the grid is sized for the longest portion and own part that the caller names: longer ones take more turns)
   for (; tile < (it.slots + per - 1) / per; tile += tiles) {
     it.first = tile * per;
-    if constexpr (FORMS == RR) rows_by_waves<D, KV8, NS, BY16>(a, it, smem, scales, apart, red);
-    else if constexpr (FORMS == KK) keys_by_waves<D, KV8, BY16>(a, it, smem, scales, apart);
-    else if (it.own) keys_by_waves<D, KV8, BY16>(a, it, smem, scales, apart);
-    else rows_by_waves<D, KV8, NS, BY16>(a, it, smem, scales, apart, red);
+    if constexpr (FORM == ROWS) rows_by_waves<D, KV8, NS, BY16>(a, it, smem, scales, apart, red);
+    else keys_by_waves<D, KV8, BY16>(a, it, smem, scales, apart);
     if (!it.own) break;
   }
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void attn_shared_join_kernel(const SharedAttn a, bf16_t* __restrict__ out, int64_t out_stride) {
+__global__ __launch_bounds__(256) void attn_shared_join_kernel(const SharedAttn a) {
   constexpr int PER = D / 4;  // threads of a (row, head)
-  const int np = a.pre_split + a.own_split;
   const int64_t i = (int64_t)blockIdx.x * (256 / PER) + threadIdx.x / PER;
   const int d = threadIdx.x % PER * 4;
   if (i >= (int64_t)a.T * a.nh) return;
   const int t = i / a.nh, h = i % a.nh;
   if (seq_of(a, t) < 0) return;  // a row of no sequence stays as it was
-  const float* ml = a.pml + i * np * 2;
-  const float* po = a.po + i * np * D + d;
-  float top = kFloor, l = 0.f;
-  for (int p = 0; p < np; ++p) top = fmaxf(top, ml[2 * p]);
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < np; ++p) {
-    const float lp = ml[2 * p + 1];
-    if (lp == 0.f) continue;  // (a part without a visible key)
-    const float f = __builtin_amdgcn_exp2f(ml[2 * p] - top);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(po + (int64_t)p * D);
-    l += lp * f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += x[e] * f;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  u16x4 r;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) r[e] = f2bf(o[e] * inv);
-  *reinterpret_cast<u16x4*>(out + (int64_t)t * out_stride + (int64_t)h * D + d) = r;
+  Joined j;
+  j.add_parts<D>(a.pml + i * a.parts * 2, a.po + i * a.parts * D + d, a.parts);
+  j.store(a.out + (int64_t)t * a.out_stride + (int64_t)h * D + d);
 }
 
 struct Plan {
@@ -715,16 +777,15 @@ int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int max_own) {
   Plan p;
-  p.ns = 1;
-  const int per = 64 * p.ns;
   const int64_t slots = (int64_t)T * G;
   p.pre_few = slots <= 16;
-  p.pre_tiles = p.pre_few ? 1 : up(slots, per);
+  p.ns = D <= 128 && slots > 64 && up(slots, 64) * 6 > up(slots, 128) * 10 ? 2 : 1;
   const int tile = tile_keys(D);
+  p.pre_tiles = up(slots, p.pre_few ? 16 : 64 * p.ns);
   if (P > 0) {
     const int unit = p.pre_few ? 128 : tile;  // keys that a workgroup takes at a time
     const int runs = up(512, (int64_t)p.pre_tiles * nkv);
-    const int want = std::max(1, std::min(runs, up(P, 2 * unit)));
+    const int want = std::max(1, std::min(runs, up(P, p.pre_few ? unit : 256)));
     p.pre_keys = up(up(P, want), unit) * unit;
     p.pre_split = up(P, p.pre_keys);
   } else {
@@ -733,7 +794,7 @@ Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int m
   }
   const int64_t portion = (int64_t)std::max(1, max_qlen) * G;
   p.own_few = p.pre_few || portion <= 16 || max_qlen == 1;
-  p.own_tiles = up(portion, p.own_few ? 16 : per);
+  p.own_tiles = up(portion, p.own_few ? 16 : 64 * p.ns);
   const int unit = p.own_few ? 128 : tile;
   const int runs = up(512, (int64_t)B * nkv * p.own_tiles);
   const int want = std::max(1, std::min(runs, up(std::max(1, max_own), 2 * unit)));
@@ -775,7 +836,8 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
   a.nkv = nkv;
   a.G = nh / nkv;
   a.bs = bs;
-  a.shift = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
+  a.shift = __builtin_ctz(bs);
+  a.page_bytes = (int64_t)nkv * bs * (kv8 ? D + kTail : 2 * D);
   a.pages = pages;
   a.P = P;
   a.own_cap = (int)std::min<int64_t>((int64_t)bt_width * bs, INT_MAX / 2);
@@ -788,30 +850,42 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
   a.own_keys = p.own_keys;
   a.own_few = p.own_few;
   a.scale_log2 = scale * kLog2eS;
+  a.out = (bf16_t*)out;
+  a.out_stride = out_stride;
+  a.parts = parts;
+  a.finish = 0;
   const int64_t pre = (int64_t)p.pre_tiles * nkv * p.pre_split, own = (int64_t)B * nkv * p.own_tiles * p.own_split;
   const int64_t join = ((int64_t)T * nh * (D / 4) + 255) / 256;
   if (pre + own > INT_MAX || join > INT_MAX || (int64_t)T * (nh / nkv) > INT_MAX / 2) throw std::runtime_error("attn_shared: too many rows");
-  a.pre_items = (int)pre;
-  const unsigned grid = (unsigned)(pre + own);
-  const int forms = p.pre_few ? KK : p.own_few ? RK : RR;
-#define SA(D_, KV8_, NS_, F_, BY_) attn_shared_kernel<D_, KV8_, NS_, F_, BY_><<<grid, 256, 0, st>>>(a)
-#define SB(D_, KV8_, NS_, F_)                  \
-  do {                                         \
-    if (bs % 16 == 0) SA(D_, KV8_, NS_, F_, true); \
-    else SA(D_, KV8_, NS_, F_, false);         \
+  // one launch for both parts where they take the same form; else the own parts', which follow, join the prefix's results themselves
+  // where each is one workgroup's
+  const bool apart = p.own_few && !p.pre_few && pre > 0;
+  const bool by16 = bs >= 16 && (bs & (bs - 1)) == 0;
+#define SA(D_, KV8_, NS_, F_, N_)                                                                 \
+  do {                                                                                            \
+    if (by16) attn_shared_kernel<D_, KV8_, NS_, F_, true><<<(unsigned)(N_), 256, 0, st>>>(a); \
+    else attn_shared_kernel<D_, KV8_, NS_, F_, false><<<(unsigned)(N_), 256, 0, st>>>(a);         \
+    HIP_CHECK_LAUNCH();                                                                           \
   } while (0)
-#define SF(D_, KV8_, NS_)                      \
-  do {                                         \
-    if (forms == RR) SB(D_, KV8_, NS_, RR);    \
-    else if (forms == RK) SB(D_, KV8_, NS_, RK); \
-    else SB(D_, KV8_, 1, KK);                  \
+#define SF(D_, KV8_, NS_)                            \
+  do {                                               \
+    a.pre_items = (int)pre;                          \
+    if (apart) {                                     \
+      SA(D_, KV8_, NS_, ROWS, pre);                  \
+      a.pre_items = 0;                               \
+      a.finish = p.own_split == 1;                   \
+      SA(D_, KV8_, 1, KEYS, own);                    \
+    } else if (p.own_few) SA(D_, KV8_, 1, KEYS, pre + own); \
+    else SA(D_, KV8_, NS_, ROWS, pre + own);         \
   } while (0)
 #define SD(D_)                                                                                    \
   do {                                                                                            \
-    if (kv8) SF(D_, true, 1);                                                                     \
+    constexpr int TWO = D_ <= 128 ? 2 : 1; /* (no such kernel for heads of 256) */                \
+    if (kv8 && p.ns == 2) SF(D_, true, TWO);                                                      \
+    else if (kv8) SF(D_, true, 1);                                                                \
+    else if (p.ns == 2) SF(D_, false, TWO);                                                       \
     else SF(D_, false, 1);                                                                        \
-    HIP_CHECK_LAUNCH();                                                                           \
-    attn_shared_join_kernel<D_><<<(unsigned)join, 256, 0, st>>>(a, (bf16_t*)out, out_stride);     \
+    if (!a.finish) attn_shared_join_kernel<D_><<<(unsigned)join, 256, 0, st>>>(a);                \
   } while (0)
   switch (D) {
     case 64: SD(64); break;
@@ -821,7 +895,6 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
   }
 #undef SD
 #undef SF
-#undef SB
 #undef SA
   HIP_CHECK_LAUNCH();
 }
