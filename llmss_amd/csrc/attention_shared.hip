@@ -25,6 +25,7 @@
 // they are kept from the slots that do not see them (see `add_values`).
 // fp8 cache rows: e4m3 numbers are exact in bf16, a row's scale multiplies its score and its weight.
 #include "common.h"
+#include <cstdlib>
 
 #include <type_traits>
 
@@ -216,20 +217,19 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS],
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        pf[n][kt >> 1][(kt & 1) * 4 + i] = (short)f2bf(__builtin_amdgcn_exp2f(fmaf(s[n][kt][i], scale_log2, nm)));
+      for (int i = 0; i < 4; ++i) {
+        s[n][kt][i] = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i], scale_log2, nm));
+        pf[n][kt >> 1][(kt & 1) * 4 + i] = (short)f2bf(s[n][kt][i]);
+      }
 #pragma unroll
     for (int k = 0; k < KT / 2; ++k) lsum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[n][k], lsum[n], 0, 0, 0);
-    if (vscale) {  // (fp8 rows: the second rounding of a weight, to half a step again)
+    if (vscale) {  // (fp8 rows: a weight times its row's scale, rounded once for the product and once for the sum)
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         const f32x4 v = *reinterpret_cast<const f32x4*>(vscale + kt * 16 + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // a key that weighs nothing is not seen, or as good as that: its scale may be anything
-          const short p = pf[n][kt >> 1][(kt & 1) * 4 + i];
-          pf[n][kt >> 1][(kt & 1) * 4 + i] = p ? (short)f2bf(__builtin_amdgcn_exp2f(fmaf(s[n][kt][i], scale_log2, nm)) * v[i]) : (short)0;
-        }
+        for (int i = 0; i < 4; ++i)  // a key that weighs nothing is not seen, or as good as that: its scale may be anything
+          pf[n][kt >> 1][(kt & 1) * 4 + i] = s[n][kt][i] != 0.f ? (short)f2bf(s[n][kt][i] * v[i]) : (short)0;
       }
     }
   }
@@ -303,20 +303,20 @@ struct Joined {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = o[e] * f + x[e] * h;
   }
-  // parts that lie one after the other, eight asked for at a time
-  template <int D>
+  // parts that lie one after the other, N asked for at a time
+  template <int D, int N>
   __device__ __forceinline__ void add_parts(const float* ml, const float* x, int n) {
-    for (int p = 0; p < n; p += 8) {
-      f32x2 b[8];
-      f32x4 v[8];
+    for (int p = 0; p < n; p += N) {
+      f32x2 b[N];
+      f32x4 v[N];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < N; ++i) {
         const int q = min(p + i, n - 1);
         b[i] = *reinterpret_cast<const f32x2*>(ml + 2 * q);
         v[i] = *reinterpret_cast<const f32x4*>(x + (int64_t)q * D);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < N; ++i)
         if (p + i < n) add(b[i], v[i]);
     }
   }
@@ -328,6 +328,36 @@ struct Joined {
     *reinterpret_cast<u16x4*>(out) = r;
   }
 };
+
+// Parts first, first + step, .. < n of a slot join what its lanes hold of it (x: the lane's first dims of the first part).
+template <int D>
+__device__ __forceinline__ void add_parts(const float* ml, const float* x, int first, int step, int n, f32x4 (&o)[D / 16], float& m, f32x4& lsum) {
+  f32x4 v[D / 16];
+  f32x2 b = {kFloor, 0.f};
+  auto load = [&](int p) {
+    b = *reinterpret_cast<const f32x2*>(ml + 2 * p);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) v[dt] = *reinterpret_cast<const f32x4*>(x + (int64_t)p * D + dt * 16);
+  };
+  if (first < n) load(first);
+#pragma unroll 1
+  for (int p = first; p < n; p += step) {
+    f32x4 w[D / 16];
+    const f32x2 c = b;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) w[dt] = v[dt];
+    if (p + step < n) load(p + step);
+    if (c[1] == 0.f) continue;  // (a part without a visible key; its outputs may be anything)
+    const float t = fmaxf(m, c[0]), f = __builtin_amdgcn_exp2f(m - t), h = __builtin_amdgcn_exp2f(c[0] - t);
+    m = t;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) lsum[e] = lsum[e] * f + c[1] * h;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[dt][e] = o[dt][e] * f + w[dt][e] * h;
+  }
+}
 
 template <int D>
 __device__ __forceinline__ void leave(const SharedAttn& a, const Item& it, int slot, int g, const f32x4 (&o)[D / 16], float m, float l) {
@@ -349,7 +379,13 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
   constexpr int BKV = tile_keys(D), KT = BKV / 16;
   constexpr int CH = D / 8;          // 16-byte chunks of an LDS row
   constexpr int TILE = BKV * D * 2;  // bytes of a tile of keys, and of values
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // (a lane's number as something new each time: what follows from it is formed where it is used and holds no registers in between)
+  auto anew = [&]() {
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  const int lane = anew(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, g = lane >> 4;
   int slot[NS], lim[NS];
   int lo = INT_MAX, hi = 0;
@@ -401,8 +437,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
     u32x4 k8[KV8 ? PIECES : 1], v8[KV8 ? PIECES : 1];
     float sc = 0.f;
     auto fetch = [&](int j) {
-      int lane = threadIdx.x & 63;
-      asm volatile("" : "+v"(lane));  // (what follows from it is formed here and holds no registers in between)
+      const int lane = anew();
       const int kv0 = it.begin + j * BKV;
       char* sk = smem + (j & 1) * 2 * TILE;
       if constexpr (KV8) {
@@ -522,8 +557,10 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
     }
   }
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
-    if (slot[n] < it.slots) leave<D>(a, it, slot[n], g, o[n], m[n], lsum[n][0]);
+  for (int n = 0; n < NS; ++n) {
+    const int l = anew(), slot = it.first + (w * NS + n) * 16 + (l & 15);
+    if (slot < it.slots) leave<D>(a, it, slot, l >> 4, o[n], m[n], lsum[n][0]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------ keys by waves
@@ -534,13 +571,28 @@ template <int D, bool KV8, bool BY16>
 __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char* smem, float* scales, bf16_t* apart) {
   constexpr int KT = 2, BK = 32, CH = D / 8;
   constexpr int TILE = BK * D * 2;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // (a lane's number as something new each time: what follows from it is formed where it is used and holds no registers in between)
+  auto anew = [&]() {
+    int l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  const int lane = anew(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, g = lane >> 4;
   const int slot = it.first + li;
   const bool real = slot < it.slots;
-  int lim[1] = {INT_MAX};
-  if (real) lim[0] = slot_limit(a, it, slot);
-  const int lo = wave_min(lim[0]), hi = wave_max(real ? lim[0] : 0);
+  Rows<BY16, KT, KV8 ? D + kTail : 2 * D> rows{a, it};
+  const int step = 4 * BK;
+  int kv0 = it.begin + w * BK;
+  rows.ask(kv0);  // (beside the context's length: a page past it is not used)
+  int lim[1] = {INT_MAX}, lo, hi;
+  if (it.own && it.slots == a.G) {  // one token: a limit for all
+    lim[0] = lo = hi = __builtin_amdgcn_readfirstlane(slot_limit(a, it, 0));
+  } else {
+    if (real) lim[0] = slot_limit(a, it, slot);
+    lo = wave_min(lim[0]);
+    hi = wave_max(real ? lim[0] : 0);
+  }
   it.stop = min(it.stop, hi);
 
   f32x4 o[1][D / 16], lsum[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
@@ -548,8 +600,6 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) o[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   __syncthreads();  // (a workgroup may have had an item before: the places below are free)
-  const int step = 4 * BK;
-  int kv0 = it.begin + w * BK;
   if (kv0 < it.stop) {
     s16x8 qf[D / 32];
     {
@@ -559,7 +609,6 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       for (int ks = 0; ks < D / 32; ++ks)
         qf[ks] = *reinterpret_cast<const s16x8*>(qp + (KV8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g));
     }
-    Rows<BY16, KT, KV8 ? D + kTail : 2 * D> rows{a, it};
     char* const img = smem + w * TILE;
     float* const fac = scales + w * 2 * BK;  // (fp8) scales of the keys, of the values
     s16x8 kf[KT][KV8 ? 1 : D / 32];
@@ -567,12 +616,6 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
     constexpr int RPI = 64 / CH, INS = BK / RPI, PIECES = BK * (D / 16) / 64;
     u32x4 v8[KV8 ? PIECES : 1];
     float sc = 0.f;
-    // (a lane's number as something new each time: what follows from it is formed where it is used and holds no registers in between)
-    auto anew = [&]() {
-      int l = lane;
-      asm volatile("" : "+v"(l));
-      return l;
-    };
     auto keys = [&](int kv0, const int (&pg)[KT]) {
       const int l = anew(), li = l & 15, g = l >> 4;
 #pragma unroll
@@ -610,17 +653,14 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       for (int i = 0; i < KT; ++i) pg[i] = rows.page(i);
       rows.ask(kv0 + step);
     };
-    rows.ask(kv0);
-    pages(kv0);
-    keys(kv0, pg);
-    values(kv0, pg);
-#pragma unroll
-    for (int ks = 0; ks < D / 32; ++ks) landed(qf[ks]);
+#pragma unroll 1
     for (; kv0 < it.stop; kv0 += step) {
-      const int nx = kv0 + step;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this run's keys and values
-      pages(nx);
-      asm volatile("" ::: "memory");
+      pages(kv0);
+      keys(kv0, pg);
+      values(kv0, pg);
+      __builtin_amdgcn_sched_barrier(0);  // (no product, and no wait for its keys, between the loads)
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
       if constexpr (KV8) {
         const int lane = anew();
 #pragma unroll
@@ -646,10 +686,6 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
           s[0][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, qf[ks], s[0][kt], 0, 0, 0);
         }
       __builtin_amdgcn_sched_barrier(0);
-      if (nx < it.stop) {  // the next run's keys come while this one's values are used
-        keys(nx, pg);
-        if constexpr (KV8) values(nx, pg);
-      }
       if constexpr (KV8) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
@@ -664,26 +700,32 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       soften<D, KT, 1, true>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
       const int l = anew();
       add_values<D, KT, 1>(kv0 + BK > min(lo, it.stop), img, apart + w * 16 * BK, left, l >> 4, l & 15, pf, o);
-      if (nx < it.stop) {
-        if constexpr (!KV8) {
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the place is read)
-          values(nx, pg);
-        }
-      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the place is read)
     }
+  }
+  const bool finish = it.own && a.finish;
+  if (finish) {  // the own part is one workgroup's: the prefix's parts, left by the launch before, join it here, every fourth a wave
+    const int l = anew(), slot = it.first + (l & 15), g = l >> 4;
+    const int sl = min(slot, it.slots - 1);
+    const int64_t pi = ((int64_t)(it.row0 + sl / a.G) * a.nh + it.kvh * a.G + sl % a.G) * a.parts;
+    add_parts<D>(a.pml + pi * 2, a.po + pi * D + 4 * g, w, 4, a.pre_split, o[0], m[0], lsum[0]);
   }
   // the waves meet: outputs [wave][slot][D] and (m, l)
   __syncthreads();
   float* const so = reinterpret_cast<float*>(smem);
   constexpr int LDO = D + 4;
+  {
+    const int l = anew(), li = l & 15, g = l >> 4;
 #pragma unroll
   for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(so + (w * 16 + li) * LDO + dt * 16 + 4 * g) = o[0][dt];
   if (g == 0) {
     scales[(w * 16 + li) * 2] = m[0];
     scales[(w * 16 + li) * 2 + 1] = lsum[0][0];
   }
+  }
   __syncthreads();
-  for (int c = threadIdx.x; c < 16 * (D / 4); c += 256) {
+#pragma unroll 1
+  for (int c = w * 64 + anew(); c < 16 * (D / 4); c += 256) {
     const int sl = c / (D / 4), d4 = c % (D / 4);
     if (it.first + sl >= it.slots) continue;
     Joined j;
@@ -692,9 +734,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       j.add(*reinterpret_cast<const f32x2*>(scales + (i * 16 + sl) * 2), *reinterpret_cast<const f32x4*>(so + (i * 16 + sl) * LDO + d4 * 4));
     const int s_ = it.first + sl;
     const int64_t row = it.row0 + s_ / a.G, head = it.kvh * a.G + s_ % a.G;
-    if (it.own && a.finish) {  // the own part is one workgroup's: the prefix's parts, left by the launch before, join it here
-      const int64_t pi = (row * a.nh + head) * a.parts;
-      j.add_parts<D>(a.pml + pi * 2, a.po + pi * D + d4 * 4, a.pre_split);
+    if (finish) {
       j.store(a.out + row * a.out_stride + head * D + d4 * 4);
     } else {
       const int64_t pi = (row * a.nh + head) * a.parts + it.part;
@@ -709,7 +749,7 @@ enum Form { ROWS, KEYS };
 // Items [0, pre_items) are the prefix's, the others own parts. The second form is bound by memory and takes few registers and little LDS:
 // more of its workgroups share a compute unit.
 template <int D, bool KV8, int NS, int FORM, bool BY16>
-__global__ __launch_bounds__(256, FORM == KEYS ? (D == 64 ? 4 : D == 128 ? 3 : 2) : 2) void attn_shared_kernel(const SharedAttn a) {
+__global__ __launch_bounds__(256, FORM == KEYS && D < 256 ? 4 : 2) void attn_shared_kernel(const SharedAttn a) {
   constexpr int PLACES = FORM == ROWS ? 2 * 2 * tile_keys(D) * D * 2 : 4 * 32 * D * 2;  // tiles; each wave's values
   constexpr int MEET = FORM == ROWS ? 0 : 4 * 16 * (D + 4) * 4;                         // the second form's outputs
   __shared__ __attribute__((aligned(16))) char smem[PLACES > MEET ? PLACES : MEET];
@@ -765,7 +805,9 @@ __global__ __launch_bounds__(256) void attn_shared_join_kernel(const SharedAttn 
   const int t = i / a.nh, h = i % a.nh;
   if (seq_of(a, t) < 0) return;  // a row of no sequence stays as it was
   Joined j;
-  j.add_parts<D>(a.pml + i * a.parts * 2, a.po + i * a.parts * D + d, a.parts);
+  const float *ml = a.pml + i * a.parts * 2, *x = a.po + i * a.parts * D + d;
+  if (a.parts <= 2) j.add_parts<D, 2>(ml, x, a.parts);
+  else j.add_parts<D, 8>(ml, x, a.parts);
   j.store(a.out + (int64_t)t * a.out_stride + (int64_t)h * D + d);
 }
 
@@ -780,11 +822,12 @@ Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int m
   const int64_t slots = (int64_t)T * G;
   p.pre_few = slots <= 16;
   p.ns = D <= 128 && slots > 64 && up(slots, 64) * 6 > up(slots, 128) * 10 ? 2 : 1;
+  if (getenv("T_NS")) p.ns = D <= 128 ? atoi(getenv("T_NS")) : 1;
   const int tile = tile_keys(D);
   p.pre_tiles = up(slots, p.pre_few ? 16 : 64 * p.ns);
   if (P > 0) {
     const int unit = p.pre_few ? 128 : tile;  // keys that a workgroup takes at a time
-    const int runs = up(512, (int64_t)p.pre_tiles * nkv);
+    const int runs = (getenv("T_WG") ? atoi(getenv("T_WG")) : 512) / ((int64_t)p.pre_tiles * nkv);  // (two workgroups a compute unit, all at once)
     const int want = std::max(1, std::min(runs, up(P, p.pre_few ? unit : 256)));
     p.pre_keys = up(up(P, want), unit) * unit;
     p.pre_split = up(P, p.pre_keys);
@@ -796,7 +839,7 @@ Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int m
   p.own_few = p.pre_few || portion <= 16 || max_qlen == 1;
   p.own_tiles = up(portion, p.own_few ? 16 : 64 * p.ns);
   const int unit = p.own_few ? 128 : tile;
-  const int runs = up(512, (int64_t)B * nkv * p.own_tiles);
+  const int runs = up(getenv("T_OWN") ? atoi(getenv("T_OWN")) : 512, (int64_t)B * nkv * p.own_tiles);
   const int want = std::max(1, std::min(runs, up(std::max(1, max_own), 2 * unit)));
   p.own_keys = up(up(std::max(1, max_own), want), unit) * unit;
   p.own_split = up(std::max(1, max_own), p.own_keys);
