@@ -25,7 +25,6 @@
 // they are kept from the slots that do not see them (see `add_values`).
 // fp8 cache rows: e4m3 numbers are exact in bf16, a row's scale multiplies its score and its weight.
 #include "common.h"
-#include <cstdlib>
 
 #include <type_traits>
 
@@ -119,6 +118,10 @@ struct Rows {
   }
   // 16 bytes a lane from memory into LDS (lane l at lds + 16 l). Through inline assembly, so that the compiler does not hold reads
   // of other places in LDS back until it has landed: every use stands behind a wait for vmcnt(0) of its own.
+  __device__ __forceinline__ void to_lds(const char* p, unsigned off, char* lds) const {  // (all of a run's rows: p the run's, off a lane's)
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LDS_AS char*)lds);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory");
+  }
   __device__ __forceinline__ void to_lds(const void* cache, int pg, int kv0, int run, int r, unsigned more, char* lds) const {
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LDS_AS char*)lds);
     if constexpr (BY16) {
@@ -436,6 +439,8 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
     constexpr int PIECES = BKV * (D / 16) / 256;
     u32x4 k8[KV8 ? PIECES : 1], v8[KV8 ? PIECES : 1];
     float sc = 0.f;
+    const int lane_row = (D == 256 ? w * RPI : w * RPI & 15) + lane / CH;
+    const unsigned lane_off = lane_row * 2 * D + (swz<D>(lane % CH, lane_row) << 4);
     auto fetch = [&](int j) {
       const int lane = anew();
       const int kv0 = it.begin + j * BKV;
@@ -459,6 +464,16 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
 #pragma unroll
         for (int i = 0; i < LPW; ++i) pg[i] = rows.page((i * 4 + w) * RPI / 16);
         rows.ask(kv0 + BKV);
+        if (BY16 && kv0 + BKV <= it.stop) {  // (a lane's row in its run and its chunk are the same for every instruction but for 8 rows)
+#pragma unroll
+          for (int i = 0; i < LPW; ++i) {
+            const int inst = i * 4 + w;
+            const int64_t at = rows.run_at(pg[i], kv0, inst * RPI / 16) + (D == 256 ? (i & 1) * 8 * 2 * D : 0);
+            rows.to_lds((const char*)a.kc + at, lane_off, sk + inst * 1024);
+            rows.to_lds((const char*)a.vc + at, lane_off, sk + TILE + inst * 1024);
+          }
+          return;
+        }
 #pragma unroll
         for (int i = 0; i < LPW; ++i) {
           const int inst = i * 4 + w, r = inst * RPI + lane / CH;
@@ -817,29 +832,48 @@ struct Plan {
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int max_own) {
+// The prefix's cut for ns groups of slots a wave, and what it takes in us: two workgroups a compute unit and all of them at once, so that
+// no second round has to be waited for (one key head, 1584 slots behind 7990 positions: 525 workgroups 45 us, 500 33), each of 256 keys or
+// more. A tile of 64 keys takes 2.0 us with one group (64 slots a workgroup), 3.3 with two (128) while two workgroups share a compute
+// unit; the partial results are written and read once, at 4.5 TB/s. Two groups halve what LDS is read for, but twice the cuts fill the
+// chip with them: 128 rows of 64 heads in 8 groups behind 16381 positions 172 us with one and 141 with two, 128 rows of 32 key heads behind
+// 8000 66 and 76, one key head as above 33 and 41. fp8 rows take as long either way (their conversion is the tile's) and heads of 256
+// have no registers for two.
+double cut_prefix(Plan& p, int ns, int64_t slots, int nkv, int D, int P) {
+  const int tile = tile_keys(D);
+  p.ns = ns;
+  p.pre_tiles = up(slots, 64 * ns);
+  const int64_t pairs = (int64_t)p.pre_tiles * nkv;
+  const int runs = (int)std::max<int64_t>(1, std::min<int64_t>(512 / pairs, up(P, 256)));
+  p.pre_keys = up(up(P, runs), tile) * tile;
+  p.pre_split = up(P, p.pre_keys);
+  const double rounds = std::max(1.0, (double)pairs * p.pre_split / 512);
+  return rounds * p.pre_keys / 64 * (ns == 2 ? 3.3 : 2.0) + 2.0 * slots * nkv * (D + 2) * 4 * p.pre_split / 4.5e6;
+}
+
+Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int max_own, bool kv8) {
   Plan p;
   const int64_t slots = (int64_t)T * G;
-  p.pre_few = slots <= 16;
-  p.ns = D <= 128 && slots > 64 && up(slots, 64) * 6 > up(slots, 128) * 10 ? 2 : 1;
-  if (getenv("T_NS")) p.ns = D <= 128 ? atoi(getenv("T_NS")) : 1;
   const int tile = tile_keys(D);
-  p.pre_tiles = up(slots, p.pre_few ? 16 : 64 * p.ns);
-  if (P > 0) {
-    const int unit = p.pre_few ? 128 : tile;  // keys that a workgroup takes at a time
-    const int runs = (getenv("T_WG") ? atoi(getenv("T_WG")) : 512) / ((int64_t)p.pre_tiles * nkv);  // (two workgroups a compute unit, all at once)
-    const int want = std::max(1, std::min(runs, up(P, p.pre_few ? unit : 256)));
-    p.pre_keys = up(up(P, want), unit) * unit;
+  p.pre_few = slots <= 16;
+  p.ns = 1;
+  p.pre_tiles = 1;
+  p.pre_split = 0;
+  p.pre_keys = tile;
+  if (P > 0 && p.pre_few) {  // 32 keys a wave at a time, as many workgroups as there are keys for up to the chip's
+    const int runs = std::max(1, std::min(512 / nkv, up(P, 128)));
+    p.pre_keys = up(up(P, runs), 128) * 128;
     p.pre_split = up(P, p.pre_keys);
-  } else {
-    p.pre_keys = tile;
-    p.pre_split = 0;
+  } else if (P > 0) {
+    const double one = cut_prefix(p, 1, slots, nkv, D, P);
+    Plan two = p;
+    if (!kv8 && D <= 128 && slots > 64 && cut_prefix(two, 2, slots, nkv, D, P) < one) p = two;
   }
   const int64_t portion = (int64_t)std::max(1, max_qlen) * G;
   p.own_few = p.pre_few || portion <= 16 || max_qlen == 1;
   p.own_tiles = up(portion, p.own_few ? 16 : 64 * p.ns);
   const int unit = p.own_few ? 128 : tile;
-  const int runs = up(getenv("T_OWN") ? atoi(getenv("T_OWN")) : 512, (int64_t)B * nkv * p.own_tiles);
+  const int runs = up(512, (int64_t)B * nkv * p.own_tiles);
   const int want = std::max(1, std::min(runs, up(std::max(1, max_own), 2 * unit)));
   p.own_keys = up(up(std::max(1, max_own), want), unit) * unit;
   p.own_split = up(std::max(1, max_own), p.own_keys);
@@ -848,8 +882,8 @@ Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int m
 
 }  // namespace
 
-int attn_shared_parts(int T, int B, int nh, int nkv, int D, int P, int max_qlen, int max_own) {
-  const Plan p = shared_plan(T, B, nkv, nh / nkv, D, P, max_qlen, max_own);
+int attn_shared_parts(int T, int B, int nh, int nkv, int D, int P, int max_qlen, int max_own, bool kv8) {
+  const Plan p = shared_plan(T, B, nkv, nh / nkv, D, P, max_qlen, max_own, kv8);
   return p.pre_split + p.own_split;
 }
 
@@ -859,7 +893,7 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
                         bool kv8, hipStream_t st) {
   if (nkv <= 0 || nh % nkv) throw std::runtime_error("attn_shared: nh must be a multiple of nkv");
   if (T == 0 || B == 0) return;
-  const Plan p = shared_plan(T, B, nkv, nh / nkv, D, P, max_qlen, max_own);
+  const Plan p = shared_plan(T, B, nkv, nh / nkv, D, P, max_qlen, max_own, kv8);
   if (p.pre_split + p.own_split != parts) throw std::runtime_error("attn_shared: the workspace was made for another call");
   SharedAttn a;
   a.q = (const bf16_t*)q;
@@ -924,8 +958,7 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
 #define SD(D_)                                                                                    \
   do {                                                                                            \
     constexpr int TWO = D_ <= 128 ? 2 : 1; /* (no such kernel for heads of 256) */                \
-    if (kv8 && p.ns == 2) SF(D_, true, TWO);                                                      \
-    else if (kv8) SF(D_, true, 1);                                                                \
+    if (kv8) SF(D_, true, 1);                                                                     \
     else if (p.ns == 2) SF(D_, false, TWO);                                                       \
     else SF(D_, false, 1);                                                                        \
     if (!a.finish) attn_shared_join_kernel<D_><<<(unsigned)join, 256, 0, st>>>(a);                \

@@ -40,7 +40,7 @@ void launch_attn_extend(const void* q, int64_t q_stride, const void* k_cache, co
                         int64_t out_stride, int B, int max_qlen, int nh, int nkv, int D, int bs, float scale,
                         hipStream_t st, bool kv8, void* q8, void* s8, int window, int nsplit, int split_keys,
                         void* part_o, void* part_ml, int total);
-int attn_shared_parts(int T, int B, int nh, int nkv, int D, int P, int max_qlen, int max_own);
+int attn_shared_parts(int T, int B, int nh, int nkv, int D, int P, int max_qlen, int max_own, bool kv8);
 void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const void* vc, int pages, const void* prefix_table, int P,
                         const void* bt, int64_t bt_stride, int bt_width, const void* cu, const void* ctx, void* out, int64_t out_stride,
                         void* ws, int parts, int T, int B, int nh, int nkv, int D, int bs, int max_qlen, int max_own, float scale,
@@ -354,7 +354,7 @@ PYBIND11_MODULE(_C, m) {
      pybind11::arg("bs"), pybind11::arg("scale"), pybind11::arg("st"), pybind11::arg("kv8"), pybind11::arg("q8") = 0,
      pybind11::arg("s8") = 0, pybind11::arg("window") = 0, pybind11::arg("nsplit") = 1,
      pybind11::arg("split_keys") = 0, pybind11::arg("po") = 0, pybind11::arg("pml") = 0, pybind11::arg("total") = 0);
-  m.def("attn_shared_parts", &attn_shared_parts);  // (rows, sequences, heads, kv heads, head dim, prefix, longest portion, own part)
+  m.def("attn_shared_parts", &attn_shared_parts);  // (rows, sequences, heads, kv heads, head dim, prefix, longest portion, own part, fp8 rows)
   m.def("attn_shared", [](uintptr_t q, int64_t qs, uintptr_t kc, uintptr_t vc, int pages, uintptr_t ptab, int P_, uintptr_t bt, int64_t bts,
                           int btw, uintptr_t cu, uintptr_t ctx, uintptr_t out, int64_t os, uintptr_t ws, int parts, int T, int B, int nh,
                           int nkv, int D, int bs, int maxq, int maxo, float scale, bool kv8, uintptr_t st) {

@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512, kPacks = 4, kMostRun = kThreads * kPacks * 8;
 constexpr int kMostBiases = 1024;
 
 struct LogitRules {
@@ -98,6 +98,16 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
   const int mrow = a.mask ? (a.mask_rows ? a.mask_rows[b] : b) : -1;
   const unsigned* mask = mrow >= 0 && mrow < a.masks ? a.mask + (int64_t)mrow * a.ldm : nullptr;
   const bool marks = len > 0 || a.biases > 0;
+  // the logits themselves are asked for first: they come while the known tokens are walked
+  float v[VEC ? kPacks : 1][8];
+  const int n8 = n & ~7;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+      const int t = (k * kThreads + threadIdx.x) * 8;
+      if (t < n8) load8(x + t, v[k]);
+    }
+  }
   auto mark = [&](int t, unsigned v, bool add) {
     unsigned* c = W16 ? cnt + (t >> 1) : cnt + t;
     if (W16 && (t & 1)) v <<= 16;
@@ -113,11 +123,21 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
     if (threadIdx.x == 0) twice = 0;
     __syncthreads();
     const int prompt = a.prompts ? min(max(a.prompts[b], 0), len) : 0;
-    for (int i = threadIdx.x; i < len; i += kThreads) {
-      const int64_t t = (a.wide ? ((const int64_t*)a.ids)[b * a.ldi + i] : (int64_t)((const int*)a.ids)[b * a.ldi + i]) - lo;
-      if (t < 0 || t >= n) continue;
-      if (i >= prompt) mark((int)t, 1u, true);
-      else mark((int)t, kSeen, false);
+    for (int i0 = threadIdx.x; i0 < len; i0 += 4 * kThreads) {
+      int64_t t[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = min(i0 + k * kThreads, len - 1);
+        t[k] = a.wide ? ((const int64_t*)a.ids)[b * a.ldi + i] : (int64_t)((const int*)a.ids)[b * a.ldi + i];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * kThreads;
+        t[k] -= lo;
+        if (i >= len || t[k] < 0 || t[k] >= n) continue;
+        if (i >= prompt) mark((int)t[k], 1u, true);
+        else mark((int)t[k], kSeen, false);
+      }
     }
     // each biased token of the run gets a place in the table; the first of its entries owns it
     const int* bi = a.bias_ids + (int64_t)b * a.ldb;
@@ -174,10 +194,10 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
   if constexpr (!VEC) {
     for (int t = threadIdx.x; t < n; t += kThreads) one(t);
   } else {
-    const int n8 = n & ~7;
-    for (int t = threadIdx.x * 8; t < n8; t += kThreads * 8) {
-      float v[8];
-      load8(x + t, v);
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+      const int t = (k * kThreads + threadIdx.x) * 8;
+      if (t >= n8) break;
       unsigned open = 0xff;
       if (mask) open = mask[(lo + t) >> 5] >> ((lo + t) & 31);
       if (marks) {
@@ -202,12 +222,12 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
         if (any) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (c[i]) v[i] = rules(v[i], c[i], t + i);
+            if (c[i]) v[k][i] = rules(v[k][i], c[i], t + i);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = open >> i & 1 ? v[i] : -INFINITY;
-      store8(y + t, v);
+      for (int i = 0; i < 8; ++i) v[k][i] = open >> i & 1 ? v[k][i] : -INFINITY;
+      store8(y + t, v[k]);
     }
     for (int t = n8 + threadIdx.x; t < n; t += kThreads) one(t);
   }
@@ -217,7 +237,7 @@ template <typename TI, typename TO>
 void launch_rules(const LogitRules& a, int B, bool w16, hipStream_t st) {
   const bool vec = ((uintptr_t)a.x | (uintptr_t)a.y) % 16 == 0 && a.ldx * sizeof(TI) % 16 == 0 && a.ldy * sizeof(TO) % 16 == 0;
   int CH = 1024;
-  while (CH < (w16 ? 16384 : 8192) && (int64_t)B * ((a.V + CH - 1) / CH) > 1024) CH *= 2;
+  while (CH < (w16 ? kMostRun : kMostRun / 2) && (int64_t)B * ((a.V + CH - 1) / CH) > 1024) CH *= 2;
   const dim3 grid((a.V + CH - 1) / CH, B);
   const size_t lds = (size_t)(w16 ? CH * 2 : CH * 4) + (size_t)a.table * 12;
 #define LR(W_, V_) adjust_logits_kernel<TI, TO, W_, V_><<<grid, kThreads, lds, st>>>(a, CH)

@@ -5,8 +5,8 @@
 // Bound by memory: the logits are read once. A workgroup owns a run of a row's tokens in registers and leaves its maximum, its sum
 // of exponentials, how many of its tokens are ahead of the given one, and its own n likeliest in order; a second launch joins a row's
 // runs. The n likeliest of a run: a number that at least n tokens reach is found from the lanes' own maxima (a binary search over the
-// bits of an order-preserving key, by ballots), and the few tokens that reach it are ranked by counting. Keys carry the token behind the
-// value, so no two are equal and a run of equal logits makes no list overflow. A NaN counts as no candidate, and makes its row's
+// upper bits of an order-preserving key, by ballots), and the few tokens that reach it are ranked by counting. Keys carry the token behind
+// the value, so no two are equal: where a run of equal logits has more than the short list takes, the search goes on over all bits. A NaN counts as no candidate, and makes its row's
 // log-probabilities NaN; a row of nothing but -inf has log-probabilities of -inf.
 #include "common.h"
 
@@ -34,22 +34,22 @@ __device__ __forceinline__ float at(const T* p) {
   else return *p;
 }
 
+// Lists of a run's likeliest hold this many keys; a run of ties that has more takes the exact way, whose list is at most kNT x 8 PACKS long.
+constexpr int kShort = 512;
+
 // NT threads, PACKS x 8 tokens a thread. Partial results of run c of row b: part[b][c] = (m, s, ahead, -), top[b][c][n] keys.
 template <typename T, int NT, int PACKS, bool VEC>
 __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ tokens, int V,
-                                                           int n, float* __restrict__ part, u64* __restrict__ top) {
+                                                           int n, int cap, float* __restrict__ part, u64* __restrict__ top) {
   constexpr int NW = NT / 64, RUN = NT * PACKS * 8;
   const int b = blockIdx.y, c = blockIdx.x, runs = gridDim.x, lo = c * RUN;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const T* row = logits + (int64_t)b * ld;
-  __shared__ float red[NW], reds[NW];
-  __shared__ int redn[NW];
+  __shared__ float red[NW], reds[NW], line[NW];
+  __shared__ int redn[NW], found;
   __shared__ u64 low[NW];
-  __shared__ int found;
-  extern __shared__ __attribute__((aligned(16))) u64 list[];  // at most n threads of a wave reach the number, 8 PACKS keys each
+  extern __shared__ __attribute__((aligned(16))) u64 list[];  // cap keys
   const int64_t tok = tokens ? tokens[b] : -1;
-  const bool given = tok >= 0 && tok < V;
-  const float mine = given ? at(row + tok) : INFINITY;
   float x[PACKS][8];
 #pragma unroll
   for (int k = 0; k < PACKS; ++k) {
@@ -72,6 +72,8 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
       for (int i = 0; i < 8; ++i) x[k][i] = t + i < V ? at(row + t + i) : -INFINITY;
     }
   }
+  const bool given = tok >= 0 && tok < V;
+  const float mine = given ? at(row + tok) : INFINITY;
   float m = -INFINITY;
   int ahead = 0;
 #pragma unroll
@@ -81,15 +83,8 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
       m = fmaxf(m, x[k][i]);
       ahead += x[k][i] > mine;
     }
-  // the run's maximum, sum and count
-  float wm = warp_max(m);
-  if (lane == 0) red[w] = wm;
-  if (threadIdx.x == 0) found = 0;
-  __syncthreads();
-  float M = red[0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) M = fmaxf(M, red[i]);
-  const float base = M == -INFINITY ? 0.f : M;
+  // the wave's maximum, and its sum against it (the waves' are joined at the end)
+  const float wm = warp_max(m), base = wm == -INFINITY ? 0.f : wm;
   constexpr float kL2e = 1.4426950408889634f;
   float s = 0.f;
 #pragma unroll
@@ -100,46 +95,79 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) ahead += __shfl_xor(ahead, o, 64);
   if (lane == 0) {
+    red[w] = wm;
     reds[w] = s;
     redn[w] = ahead;
   }
-  // a number that n of the wave's lanes reach with their best token (0: fewer have one)
   if (n > 0) {
-    u64 best = 0;
+    // a value that n of the wave's lanes reach with their best (-inf: fewer do), to the upper 16 bits of its key
+    const unsigned best = (unsigned)(key_of(m, 0) >> 32);
+    unsigned reach = 0;
 #pragma unroll
-    for (int k = 0; k < PACKS; ++k)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int t = lo + (k * NT + threadIdx.x) * 8 + i;
-        const u64 q = t < V ? key_of(x[k][i], t) : 0ull;
-        best = q > best ? q : best;
-      }
-    u64 reach = 0;
-#pragma unroll 1
-    for (int bit = 63; bit >= 0; --bit) {
-      const u64 want = reach | 1ull << bit;
+    for (int bit = 31; bit >= 16; --bit) {
+      const unsigned want = reach | 1u << bit;
       if (__popcll(__ballot(best >= want)) >= n) reach = want;
     }
-    if (lane == 0) low[w] = reach;
+    if (lane == 0) line[w] = reach <= 0x007fffffu ? -INFINITY : value_of((u64)reach << 32);
+    if (threadIdx.x == 0) found = 0;
     __syncthreads();
-    u64 line = low[0];
+    float L = line[0];
 #pragma unroll
-    for (int i = 1; i < NW; ++i) line = low[i] > line ? low[i] : line;
-    if (line == 0) line = 1;
-    if (best >= line) {
+    for (int i = 1; i < NW; ++i) L = fmaxf(L, line[i]);
+    if (m >= L) {  // (a thread without a token has -inf)
+#pragma unroll
+      for (int k = 0; k < PACKS; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int t = lo + (k * NT + threadIdx.x) * 8 + i;
+          if (x[k][i] >= L && t < V) {
+            const int p = atomicAdd(&found, 1);
+            if (p < cap) list[p] = key_of(x[k][i], t);
+          }
+        }
+    }
+  }
+  __syncthreads();
+  if (n > 0) {
+    int have = found;
+    if (have > kShort) {  // (ties, or a run with few numbers: the same in every thread)
+      // the exact way: keys that hold the token too are never equal, so at most n lanes of a wave reach the line
+      u64 best = 0;
 #pragma unroll
       for (int k = 0; k < PACKS; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int t = lo + (k * NT + threadIdx.x) * 8 + i;
           const u64 q = t < V ? key_of(x[k][i], t) : 0ull;
-          if (q >= line) list[atomicAdd(&found, 1)] = q;
+          best = q > best ? q : best;
         }
+      u64 reach = 0;
+#pragma unroll 1
+      for (int bit = 63; bit >= 0; --bit) {
+        const u64 want = reach | 1ull << bit;
+        if (__popcll(__ballot(best >= want)) >= n) reach = want;
+      }
+      if (lane == 0) low[w] = reach;
+      __syncthreads();
+      if (threadIdx.x == 0) found = 0;
+      u64 l = low[0];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) l = low[i] > l ? low[i] : l;
+      if (l == 0) l = 1;
+      __syncthreads();
+      if (best >= l) {
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int t = lo + (k * NT + threadIdx.x) * 8 + i;
+            const u64 q = t < V ? key_of(x[k][i], t) : 0ull;
+            if (q >= l) list[atomicAdd(&found, 1)] = q;
+          }
+      }
+      __syncthreads();
+      have = found;
     }
-  }
-  __syncthreads();
-  if (n > 0) {
-    const int have = found;
     u64* mine_top = top + ((int64_t)b * runs + c) * n;
     for (int i = threadIdx.x; i < have; i += NT) {
       const u64 q = list[i];
@@ -150,75 +178,115 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
     for (int i = have + threadIdx.x; i < n; i += NT) mine_top[i] = 0;
   }
   if (threadIdx.x == 0) {
-    float S = 0.f;
+    float M = red[0], S = 0.f;
     int A = 0;
 #pragma unroll
+    for (int i = 1; i < NW; ++i) M = fmaxf(M, red[i]);
+#pragma unroll
     for (int i = 0; i < NW; ++i) {
-      S += reds[i];
+      // (a wave of -inf alone gives nothing; its sum may be NaN, which stays)
+      S += red[i] == -INFINITY ? reds[i] : reds[i] * __builtin_amdgcn_exp2f((red[i] - M) * kL2e);
       A += redn[i];
     }
-    float* o = part + ((int64_t)b * runs + c) * 4;
-    o[0] = M;
-    o[1] = S;
-    o[2] = __int_as_float(A);
+    *reinterpret_cast<f32x4*>(part + ((int64_t)b * runs + c) * 4) = f32x4{M, S, __int_as_float(A), 0.f};
   }
 }
 
-// One workgroup a row: the row's sum, then every run's n likeliest are placed by how many of each run are ahead of them.
+// One workgroup a row: the row's sum, then the runs' likeliest are ranked. Every run's keys stand in order, so of n keys that are wanted
+// none lies below the j-th of each run with j = n / runs, nor below any run's n-th: what is left is ranked by counting.
 template <typename T>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ tokens, int V, int n,
                                                             int runs, const float* __restrict__ part, const u64* __restrict__ top,
                                                             float* __restrict__ lp, int64_t* __restrict__ rank,
                                                             int64_t* __restrict__ top_ids, float* __restrict__ top_lp) {
-  extern __shared__ __attribute__((aligned(16))) u64 keys[];
-  __shared__ float red[32];
-  const int b = blockIdx.x;
-  const float* p = part + (int64_t)b * runs * 4;
-  for (int i = threadIdx.x; i < runs * n; i += 256) keys[i] = top[(int64_t)b * runs * n + i];
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < runs; i += 256) m = fmaxf(m, p[4 * i]);
-  const float M = block_max(m, red);
+  extern __shared__ __attribute__((aligned(16))) u64 keys[];  // runs x n, and as many that are left
+  __shared__ float redm[4], reds[4];
+  __shared__ int reda[4], redt[4], left;
+  __shared__ u64 redj[4], redn[4];
+  const int b = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  u64* const kept = keys + (int64_t)runs * n;
+  const int64_t tok = tokens ? tokens[b] : -1;
+  const bool given = tok >= 0 && tok < V;
+  const float mine = given ? at(logits + (int64_t)b * ld + tok) : 0.f;
+  const int j = n > 0 ? min((n + runs - 1) / runs, n) : 0;
+  float m = -INFINITY, s = 0.f;
+  int ahead = 0, there = 0;
+  u64 least = ~0ull, most = 0;  // of the runs' j-th keys, of their n-th ones
   constexpr float kL2e = 1.4426950408889634f;
-  float s = 0.f;
-  int ahead = 0;
   for (int i = threadIdx.x; i < runs; i += 256) {
-    const float mi = p[4 * i];
+    const f32x4 p = *reinterpret_cast<const f32x4*>(part + ((int64_t)b * runs + i) * 4);
+    const float t = fmaxf(m, p[0]);
     // (a run of -inf alone gives nothing; its sum may be NaN, which stays)
-    s += mi == -INFINITY ? (p[4 * i + 1] != p[4 * i + 1] ? NAN : 0.f) : p[4 * i + 1] * __builtin_amdgcn_exp2f((mi - M) * kL2e);
-    ahead += __float_as_int(p[4 * i + 2]);
+    s = (m == -INFINITY ? s : s * __builtin_amdgcn_exp2f((m - t) * kL2e)) + (p[0] == -INFINITY ? p[1] : p[1] * __builtin_amdgcn_exp2f((p[0] - t) * kL2e));
+    m = t;
+    ahead += __float_as_int(p[2]);
+    if (n > 0) {
+      const u64 kj = top[((int64_t)b * runs + i) * n + j - 1], kn = top[((int64_t)b * runs + i) * n + n - 1];
+      least = kj < least ? kj : least;
+      most = kn > most ? kn : most;
+    }
   }
-  const f32x2 both = block_sum2(s, 0.f, red);
-  int there = 0;
-  for (int i = threadIdx.x; i < runs * n; i += 256) there += keys[i] != 0;
-  const f32x2 counts = block_sum2((float)ahead, (float)there, red);  // (below 2^24: exact)
-  const float ls = M == -INFINITY && both[0] == 0.f ? 0.f : logf(both[0]);
-  const float base = M == -INFINITY ? 0.f : M;
+  for (int i = threadIdx.x; i < runs * n; i += 256) {
+    const u64 q = top[(int64_t)b * runs * n + i];
+    keys[i] = q;
+    there += q != 0;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), t = fmaxf(m, m2);
+    s = (m == -INFINITY ? s : s * __builtin_amdgcn_exp2f((m - t) * kL2e)) + (m2 == -INFINITY ? s2 : s2 * __builtin_amdgcn_exp2f((m2 - t) * kL2e));
+    m = t;
+    ahead += __shfl_xor(ahead, o, 64);
+    there += __shfl_xor(there, o, 64);
+    const u64 l2 = __shfl_xor(least, o, 64), n2 = __shfl_xor(most, o, 64);
+    least = l2 < least ? l2 : least;
+    most = n2 > most ? n2 : most;
+  }
+  if (lane == 0) {
+    redm[w] = m;
+    reds[w] = s;
+    reda[w] = ahead;
+    redt[w] = there;
+    redj[w] = least;
+    redn[w] = most;
+  }
+  if (threadIdx.x == 0) left = 0;
+  __syncthreads();
+  float M = redm[0], S = 0.f;
+  int A = 0, all = 0;
+  u64 line = 0, lj = ~0ull;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) M = fmaxf(M, redm[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    S += redm[i] == -INFINITY ? reds[i] : reds[i] * __builtin_amdgcn_exp2f((redm[i] - M) * kL2e);
+    A += reda[i];
+    all += redt[i];
+    lj = redj[i] < lj ? redj[i] : lj;
+    line = redn[i] > line ? redn[i] : line;
+  }
+  line = lj > line ? lj : line;
+  if (line == 0) line = 1;
+  const float base = M == -INFINITY ? 0.f : M, ls = M == -INFINITY && S == 0.f ? 0.f : logf(S);
   if (threadIdx.x == 0) {
-    const int64_t tok = tokens ? tokens[b] : -1;
-    const bool given = tok >= 0 && tok < V;
-    lp[b] = given ? at(logits + (int64_t)b * ld + tok) - base - ls : 0.f;
-    rank[b] = given ? (int64_t)counts[0] + 1 : 0;
+    lp[b] = given ? mine - base - ls : 0.f;
+    rank[b] = given ? (int64_t)A + 1 : 0;
   }
-  for (int i = (int)counts[1] + threadIdx.x; i < n; i += 256) {  // (a row of so many NaN that there are no n others)
+  if (n == 0) return;
+  for (int i = threadIdx.x; i < runs * n; i += 256) {
+    const u64 q = keys[i];
+    if (q >= line) kept[atomicAdd(&left, 1)] = q;
+  }
+  for (int i = all + threadIdx.x; i < n; i += 256) {  // (a row of so many NaN that there are no n others)
     top_ids[(int64_t)b * n + i] = -1;
     top_lp[(int64_t)b * n + i] = NAN;
   }
-  for (int i = threadIdx.x; i < runs * n; i += 256) {
-    const u64 q = keys[i];
-    if (q == 0) continue;
-    const int own = i / n;
-    int place = i - own * n;
-    for (int c = 0; c < runs; ++c) {
-      if (c == own) continue;
-      int lo = 0, hi = n;  // keys of run c above q
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (keys[c * n + mid] > q) lo = mid + 1;
-        else hi = mid;
-      }
-      place += lo;
-      if (place >= n) break;
-    }
+  __syncthreads();
+  const int have = left;
+  for (int i = threadIdx.x; i < have; i += 256) {
+    const u64 q = kept[i];
+    int place = 0;
+    for (int c = 0; c < have; ++c) place += kept[c] > q;
     if (place < n) {
       top_ids[(int64_t)b * n + place] = (int)~(unsigned)q;
       top_lp[(int64_t)b * n + place] = value_of(q) - base - ls;
@@ -234,6 +302,9 @@ int packs_of(int B, int V, int n) {
   return V > (1 << 18) || (int64_t)B * ((V + 4 * 8 * kNT - 1) / (4 * 8 * kNT)) >= 512 ? 4 : 1;
 }
 
+// Keys that a run's list holds: what the exact way may need, at most n threads of each wave.
+int list_of(int n, int packs) { return n == 0 ? 0 : std::max(kShort, std::min(4 * n, kNT) * packs * 8); }
+
 }  // namespace
 
 int logprobs_runs(int B, int V, int n) {
@@ -248,11 +319,11 @@ void launch_logprobs(const void* logits, int64_t ld, bool fp32, const void* toke
   if (n < 0 || n > kMostTop || n > V) throw std::runtime_error("token_logprobs: top_n must be between 0 and min(64, vocab)");
   const int packs = packs_of(B, V, n), runs = logprobs_runs(B, V, n);
   const size_t join = (size_t)runs * n * 8;
-  if (V >= 1 << 24 || join > 60 * 1024) throw std::runtime_error("token_logprobs: vocabulary too large");
+  if (V >= 1 << 24 || join > 30 * 1024) throw std::runtime_error("token_logprobs: vocabulary too large");
   const bool vec = (uintptr_t)logits % 16 == 0 && ld * (fp32 ? 4 : 2) % 16 == 0;
   const dim3 grid(runs, B);
 #define LK(T_, P_, V_)                                                                                                  \
-  logprobs_runs_kernel<T_, kNT, P_, V_><<<grid, kNT, std::min((size_t)n * 4, (size_t)kNT) * P_ * 8 * 8, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, \
+  logprobs_runs_kernel<T_, kNT, P_, V_><<<grid, kNT, (size_t)list_of(n, P_) * 8, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, list_of(n, P_), \
                                                                                 (float*)part, (u64*)top)
 #define LP(T_)                                                                                                          \
   do {                                                                                                                  \
@@ -267,7 +338,7 @@ void launch_logprobs(const void* logits, int64_t ld, bool fp32, const void* toke
       else LK(T_, 1, false);                                                                                            \
     }                                                                                                                   \
     HIP_CHECK_LAUNCH();                                                                                                 \
-    logprobs_join_kernel<T_><<<B, 256, join, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, runs, (const float*)part, \
+    logprobs_join_kernel<T_><<<B, 256, 2 * join, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, runs, (const float*)part, \
                                                    (const u64*)top, (float*)lp, (int64_t*)rank, (int64_t*)top_ids, (float*)top_lp); \
   } while (0)
   if (fp32) LP(float);

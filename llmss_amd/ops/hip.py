@@ -261,7 +261,7 @@ def attn_shared(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx
     if T == 0 or B == 0:
         return y
     C = lib()
-    parts = C.attn_shared_parts(T, B, nh, nkv, D, prefix_len, max_qlen, max_own)
+    parts = C.attn_shared_parts(T, B, nh, nkv, D, prefix_len, max_qlen, max_own, kv8)
     ws = torch.empty(T * nh * parts * (D + 2), dtype=torch.float32, device=q.device)
     C.attn_shared(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], prefix_table.data_ptr(),
                   prefix_len, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], _ptr(cu_q),
@@ -302,7 +302,7 @@ def token_logprobs(logits, tokens, top_n=0, vocab=None):
     dev = logits.device
     C = lib()
     runs = C.logprobs_runs(B, V, top_n)
-    _check(runs * top_n * 8 <= 60 * 1024, "vocabulary too large for so many of the likeliest tokens")
+    _check(runs * top_n * 8 <= 30 * 1024, "vocabulary too large for so many of the likeliest tokens")
     lp = torch.empty(B, dtype=torch.float32, device=dev)
     rank = torch.empty(B, dtype=torch.int64, device=dev)
     ids = torch.empty(B, top_n, dtype=torch.int64, device=dev)
