@@ -116,14 +116,12 @@ struct Rows {
     if constexpr (BY16) return *reinterpret_cast<const V*>((const char*)cache + run_at(pg, kv0, run) + (row_at(kv0, run, r) + more));
     else return *reinterpret_cast<const V*>((const char*)cache + alone(kv0 + 16 * run + r) + more);
   }
-  // 16 bytes a lane from memory into LDS (lane l at lds + 16 l). Through inline assembly, so that the compiler does not hold reads
+  // 16 bytes a lane from memory into LDS (lane l at `at` + 16 l, the same `at` in every lane). Through inline assembly, so that the compiler does not hold reads
   // of other places in LDS back until it has landed: every use stands behind a wait for vmcnt(0) of its own.
-  __device__ __forceinline__ void to_lds(const char* p, unsigned off, char* lds) const {  // (all of a run's rows: p the run's, off a lane's)
-    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LDS_AS char*)lds);
+  __device__ __forceinline__ void to_lds(const char* p, unsigned off, unsigned at) const {  // (all of a run's rows: p the run's, off a lane's)
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory");
   }
-  __device__ __forceinline__ void to_lds(const void* cache, int pg, int kv0, int run, int r, unsigned more, char* lds) const {
-    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LDS_AS char*)lds);
+  __device__ __forceinline__ void to_lds(const void* cache, int pg, int kv0, int run, int r, unsigned more, unsigned at) const {
     if constexpr (BY16) {
       const char* p = (const char*)cache + run_at(pg, kv0, run);
       const unsigned off = row_at(kv0, run, r) + more;
@@ -231,8 +229,11 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS],
       for (int kt = 0; kt < KT; ++kt) {
         const f32x4 v = *reinterpret_cast<const f32x4*>(vscale + kt * 16 + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)  // a key that weighs nothing is not seen, or as good as that: its scale may be anything
-          pf[n][kt >> 1][(kt & 1) * 4 + i] = s[n][kt][i] != 0.f ? (short)f2bf(s[n][kt][i] * v[i]) : (short)0;
+        for (int i = 0; i < 4; ++i) {
+          const short x = (short)f2bf(s[n][kt][i] * v[i]);
+          // (a key that is not seen: its scale may be anything)
+          pf[n][kt >> 1][(kt & 1) * 4 + i] = !MASK || s[n][kt][i] != 0.f ? x : (short)0;
+        }
       }
     }
   }
@@ -439,12 +440,13 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
     constexpr int PIECES = BKV * (D / 16) / 256;
     u32x4 k8[KV8 ? PIECES : 1], v8[KV8 ? PIECES : 1];
     float sc = 0.f;
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LDS_AS char*)smem);
     const int lane_row = (D == 256 ? w * RPI : w * RPI & 15) + lane / CH;
     const unsigned lane_off = lane_row * 2 * D + (swz<D>(lane % CH, lane_row) << 4);
     auto fetch = [&](int j) {
       const int lane = anew();
       const int kv0 = it.begin + j * BKV;
-      char* sk = smem + (j & 1) * 2 * TILE;
+      const unsigned sl = lds0 + (j & 1) * 2 * TILE;
       if constexpr (KV8) {
         int pg[PIECES];
 #pragma unroll
@@ -469,16 +471,16 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
           for (int i = 0; i < LPW; ++i) {
             const int inst = i * 4 + w;
             const int64_t at = rows.run_at(pg[i], kv0, inst * RPI / 16) + (D == 256 ? (i & 1) * 8 * 2 * D : 0);
-            rows.to_lds((const char*)a.kc + at, lane_off, sk + inst * 1024);
-            rows.to_lds((const char*)a.vc + at, lane_off, sk + TILE + inst * 1024);
+            rows.to_lds((const char*)a.kc + at, lane_off, sl + inst * 1024);
+            rows.to_lds((const char*)a.vc + at, lane_off, sl + TILE + inst * 1024);
           }
           return;
         }
 #pragma unroll
         for (int i = 0; i < LPW; ++i) {
           const int inst = i * 4 + w, r = inst * RPI + lane / CH;
-          rows.to_lds(a.kc, pg[i], kv0, inst * RPI / 16, r & 15, swz<D>(lane % CH, r) << 4, sk + inst * 1024);
-          rows.to_lds(a.vc, pg[i], kv0, inst * RPI / 16, r & 15, swz<D>(lane % CH, r) << 4, sk + TILE + inst * 1024);
+          rows.to_lds(a.kc, pg[i], kv0, inst * RPI / 16, r & 15, swz<D>(lane % CH, r) << 4, sl + inst * 1024);
+          rows.to_lds(a.vc, pg[i], kv0, inst * RPI / 16, r & 15, swz<D>(lane % CH, r) << 4, sl + TILE + inst * 1024);
         }
       }
     };
@@ -625,6 +627,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
         qf[ks] = *reinterpret_cast<const s16x8*>(qp + (KV8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g));
     }
     char* const img = smem + w * TILE;
+    const unsigned img_at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LDS_AS char*)img);
     float* const fac = scales + w * 2 * BK;  // (fp8) scales of the keys, of the values
     s16x8 kf[KT][KV8 ? 1 : D / 32];
     u32x4 k8[KT][KV8 ? D / 64 : 1];
@@ -658,7 +661,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
 #pragma unroll
         for (int i = 0; i < INS; ++i) {
           const int r = i * RPI + lane / CH;
-          rows.to_lds(a.vc, pg[i * RPI / 16], kv0, i * RPI / 16, r & 15, swz<D>(lane % CH, r) << 4, img + i * 1024);
+          rows.to_lds(a.vc, pg[i * RPI / 16], kv0, i * RPI / 16, r & 15, swz<D>(lane % CH, r) << 4, img_at + i * 1024);
         }
       }
     };

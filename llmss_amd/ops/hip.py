@@ -41,6 +41,10 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (  # the handle alone: building torch's stream object takes 2.6 us
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -236,11 +240,12 @@ def attn_extend(q, k_cache, v_cache, block_tables, cu_q, ctx_lens, max_qlen, nh,
 
 
 def _here(*ts):
-    """Every tensor given lies on the current device (kernels are launched on its stream)."""
+    """Every tensor given lies on the current device (kernels are launched on its stream); its index."""
     dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None and (not t.is_cuda or t.device.index != dev):
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"a tensor is on {t.device} but the current device is cuda:{dev}")
+    return dev
 
 
 def attn_shared(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx_lens, nh, nkv, D, scale, cu_q=None, max_qlen=1,
@@ -248,68 +253,66 @@ def attn_shared(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx
     """Attention behind a prefix that the whole batch shares (ops.reference.attn_shared says what it computes); csrc/attention_shared.hip.
     The partial results live in a buffer of this call's own, from the caching allocator of the current stream, so calls on several
     streams and captured graphs share none."""
-    prefix_len, max_qlen = int(prefix_len), int(max_qlen)
     B, kv8, max_own = _ref.attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx_lens, nh, nkv, D, cu_q,
                                              max_qlen, max_own, out)
-    _check(scale > 0, "scale must be positive")
-    _here(q, k_cache, v_cache, prefix_table, block_tables, ctx_lens, cu_q, out)
-    _check(q.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0, "q rows must be 16-byte aligned")
-    _check(ctx_lens.is_contiguous(), "ctx_lens must be contiguous")
+    dev = _here(q, k_cache, v_cache, prefix_table, block_tables, ctx_lens, cu_q, out)
+    qp, qs = q.data_ptr(), q.stride(0)
+    _check(qp % 16 == 0 and qs % 8 == 0 and scale > 0, "q rows must be 16-byte aligned, scale positive")
     T = q.shape[0]
-    y = out if out is not None else torch.empty(T, nh * D, dtype=q.dtype, device=q.device)
-    _check(y.data_ptr() % 8 == 0 and y.stride(0) % 4 == 0, "out rows must be 8-byte aligned")
+    y = out if out is not None else q.new_empty((T, nh * D))
+    yp, ys = y.data_ptr(), y.stride(0)
+    _check(yp % 8 == 0 and ys % 4 == 0, "out rows must be 8-byte aligned")
     if T == 0 or B == 0:
         return y
     C = lib()
     parts = C.attn_shared_parts(T, B, nh, nkv, D, prefix_len, max_qlen, max_own, kv8)
-    ws = torch.empty(T * nh * parts * (D + 2), dtype=torch.float32, device=q.device)
-    C.attn_shared(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], prefix_table.data_ptr(),
-                  prefix_len, block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], _ptr(cu_q),
-                  ctx_lens.data_ptr(), y.data_ptr(), y.stride(0), ws.data_ptr(), parts, T, B, nh, nkv, D, k_cache.shape[2],
-                  max_qlen, max_own, float(scale), kv8, _stream())
+    ws = q.new_empty(T * nh * parts * (D + 2), dtype=torch.float32)
+    nb, _, bs, _ = k_cache.shape
+    C.attn_shared(qp, qs, k_cache.data_ptr(), v_cache.data_ptr(), nb, prefix_table.data_ptr(), prefix_len, block_tables.data_ptr(),
+                  block_tables.stride(0), block_tables.shape[1], 0 if cu_q is None else cu_q.data_ptr(), ctx_lens.data_ptr(), yp, ys,
+                  ws.data_ptr(), parts, T, B, nh, nkv, D, bs, max_qlen, max_own, scale, kv8, _raw_stream(dev))
     return y
 
 
 def adjust_logits(logits, ids=None, lens=None, prompt_lens=None, repetition=None, presence=None, frequency=None, bias_ids=None,
                   bias=None, mask=None, mask_rows=None, vocab=None, out=None):
-    """Penalties, biases and masks on logits (ops.reference.adjust_logits says what it computes); csrc/logits.hip. Rows of the result
+    """Penalties, biases and masks on logits (ops.reference.adjust_logits says what it computes); csrc/logits.hip. Rows of a new result
     start on 16 bytes."""
     B, V = _ref.adjust_logits_check(logits, ids, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, mask, mask_rows,
                                     vocab, out)
-    _here(logits, ids, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, mask, mask_rows, out)
+    dev = _here(logits, ids, lens, prompt_lens, repetition, presence, frequency, bias_ids, bias, mask, mask_rows, out)
     _check(B <= 65535, "at most 65535 rows")
+    f32 = torch.float32
     if out is None:
-        y = torch.empty(B, (V + 7) // 8 * 8, dtype=logits.dtype, device=logits.device)[:, :V]
+        wide = (V + 7) // 8 * 8
+        y = logits.new_empty((B, V)) if wide == V else logits.new_empty((B, wide))[:, :V]
     else:
         y = out[:B, :V]
-    lib().adjust_logits(logits.data_ptr(), logits.stride(0), logits.dtype == torch.float32, y.data_ptr(), y.stride(0),
-                        y.dtype == torch.float32, B, V, _ptr(ids), ids.stride(0) if ids is not None else 0,
-                        ids.shape[1] if ids is not None else 0, ids is not None and ids.dtype == torch.int64, _ptr(lens),
-                        _ptr(prompt_lens), _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias_ids), _ptr(bias),
-                        bias_ids.stride(0) if bias_ids is not None else 0, bias_ids.shape[1] if bias_ids is not None else 0,
-                        _ptr(mask), mask.stride(0) if mask is not None else 0, _ptr(mask_rows),
-                        mask.shape[0] if mask is not None else 0, _stream())
+    lib().adjust_logits(logits.data_ptr(), logits.stride(0), logits.dtype == f32, y.data_ptr(), y.stride(0), y.dtype == f32, B, V,
+                        _ptr(ids), ids.stride(0) if ids is not None else 0, ids.shape[1] if ids is not None else 0,
+                        ids is not None and ids.dtype == torch.int64, _ptr(lens), _ptr(prompt_lens), _ptr(repetition), _ptr(presence),
+                        _ptr(frequency), _ptr(bias_ids), _ptr(bias), bias_ids.stride(0) if bias_ids is not None else 0,
+                        bias_ids.shape[1] if bias_ids is not None else 0, _ptr(mask), mask.stride(0) if mask is not None else 0,
+                        _ptr(mask_rows), mask.shape[0] if mask is not None else 0, _raw_stream(dev))
     return y
 
 
 def token_logprobs(logits, tokens, top_n=0, vocab=None):
     """Log-probability and rank of a token a row, and the likeliest tokens (ops.reference.token_logprobs says what it computes);
     csrc/logprobs.hip."""
-    top_n = int(top_n)
     B, V = _ref.token_logprobs_check(logits, tokens, top_n, vocab)
-    _here(logits, tokens)
+    dev = _here(logits, tokens)
     _check(B <= 65535 and V < 1 << 24, "at most 65535 rows and 2 ** 24 - 1 tokens")
-    dev = logits.device
     C = lib()
+    f32, i64 = torch.float32, torch.int64
     runs = C.logprobs_runs(B, V, top_n)
     _check(runs * top_n * 8 <= 30 * 1024, "vocabulary too large for so many of the likeliest tokens")
-    lp = torch.empty(B, dtype=torch.float32, device=dev)
-    rank = torch.empty(B, dtype=torch.int64, device=dev)
-    ids = torch.empty(B, top_n, dtype=torch.int64, device=dev)
-    tlp = torch.empty(B, top_n, dtype=torch.float32, device=dev)
-    ws = torch.empty(B * runs * (2 + top_n), dtype=torch.int64, device=dev)  # (m, s, count, -) and the likeliest of each run
-    C.token_logprobs(logits.data_ptr(), logits.stride(0), logits.dtype == torch.float32, _ptr(tokens), B, V, top_n, ws.data_ptr(),
-                     ws.data_ptr() + B * runs * 16, lp.data_ptr(), rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), _stream())
+    lp, tlp = logits.new_empty(B, dtype=f32), logits.new_empty((B, top_n), dtype=f32)
+    rank, ids = logits.new_empty(B, dtype=i64), logits.new_empty((B, top_n), dtype=i64)
+    ws = logits.new_empty(B * runs * (2 + top_n), dtype=i64)  # (m, s, count, -) and the likeliest of each run
+    wp = ws.data_ptr()
+    C.token_logprobs(logits.data_ptr(), logits.stride(0), logits.dtype == f32, _ptr(tokens), B, V, top_n, wp, wp + B * runs * 16,
+                     lp.data_ptr(), rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), _raw_stream(dev))
     return lp, rank, ids, tlp
 
 

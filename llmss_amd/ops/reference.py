@@ -241,34 +241,40 @@ def _need(cond: bool, msg: str):
 
 def attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx_lens, nh, nkv, D, cu_q, max_qlen, max_own, out):
     """What attn_shared asks of its arguments, on either device: (sequences, fp8 rows, positions that ``max_own`` stands for)."""
+    bf16, u8, i32 = torch.bfloat16, torch.uint8, torch.int32
     _need(nkv > 0 and nh > 0 and nh % nkv == 0, "nh must be a multiple of nkv")
     _need(D in (64, 128, 256), "shared-prefix attention supports head_dim 64/128/256")
-    _need(q.dim() == 2 and q.dtype == torch.bfloat16 and q.stride(1) == 1 and q.shape[1] >= nh * D, "q bf16 [T, >= nh * D]")
-    kv8 = k_cache.dtype == torch.uint8
-    _need(k_cache.dtype in (torch.bfloat16, torch.uint8) and k_cache.dim() == 4 and k_cache.shape[1] == nkv
-          and k_cache.shape[3] == (D + KV8_TAIL if kv8 else D) and k_cache.is_contiguous(),
+    _need(q.dim() == 2 and q.dtype == bf16 and q.stride(1) == 1 and q.shape[1] >= nh * D, "q bf16 [T, >= nh * D]")
+    ct = k_cache.dtype
+    kv8 = ct == u8
+    cs = k_cache.shape
+    _need((ct == bf16 or kv8) and len(cs) == 4 and cs[1] == nkv and cs[3] == (D + KV8_TAIL if kv8 else D) and k_cache.is_contiguous(),
           "k_cache bf16 [nb, nkv, bs, D] or uint8 (fp8 rows) [nb, nkv, bs, D + 16]")
-    _need(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype and v_cache.is_contiguous(), "v_cache like k_cache")
-    bs = k_cache.shape[2]
-    _need(k_cache.shape[0] > 0 and bs > 0, "an empty cache")
-    for t, n, nm in ((prefix_table, 1, "prefix_table"), (block_tables, 2, "block_tables"), (ctx_lens, 1, "ctx_lens")):
-        _need(t.dtype == torch.int32 and t.dim() == n and (t.numel() == 0 or t.stride(-1) == 1), f"{nm} must be int32, {n}-D, dense rows")
-    _need(0 <= prefix_len <= prefix_table.numel() * bs, "prefix_len must be between 0 and what prefix_table holds")
+    _need(v_cache.shape == cs and v_cache.dtype == ct and v_cache.is_contiguous(), "v_cache like k_cache")
+    bs = cs[2]
+    _need(cs[0] > 0 and bs > 0, "an empty cache")
+    _need(prefix_table.dtype == i32 and prefix_table.dim() == 1 and prefix_table.is_contiguous(), "prefix_table int32 [pages]")
+    _need(block_tables.dtype == i32 and block_tables.dim() == 2 and (block_tables.shape[1] <= 1 or block_tables.stride(1) == 1),
+          "block_tables int32 [B, pages], dense rows")
+    _need(ctx_lens.dtype == i32 and ctx_lens.dim() == 1 and ctx_lens.is_contiguous(), "ctx_lens int32 [B]")
+    _need(isinstance(prefix_len, int) and 0 <= prefix_len <= prefix_table.numel() * bs,
+          "prefix_len must be a number between 0 and what prefix_table holds")
     T = q.shape[0]
     if cu_q is None:
         B = T
         _need(max_qlen == 1, "several tokens a sequence need cu_q")
     else:
-        _need(cu_q.dtype == torch.int32 and cu_q.dim() == 1 and cu_q.numel() >= 1 and cu_q.is_contiguous(), "cu_q int32 [B + 1]")
+        _need(cu_q.dtype == i32 and cu_q.dim() == 1 and cu_q.numel() >= 1 and cu_q.is_contiguous(), "cu_q int32 [B + 1]")
         B = cu_q.numel() - 1
-        _need(max_qlen >= 1, "max_qlen")
-    _need(ctx_lens.numel() >= B and block_tables.shape[0] >= B, "ctx_lens and block_tables need a row for each sequence")
-    room = block_tables.shape[1] * bs
+        _need(isinstance(max_qlen, int) and max_qlen >= 1, "max_qlen")
+    rows, cols = block_tables.shape
+    _need(ctx_lens.numel() >= B and rows >= B, "ctx_lens and block_tables need a row for each sequence")
+    room = cols * bs
     if max_own is None:
         max_own = room
-    _need(0 <= max_own <= room, "max_own must be between 0 and what a row of block_tables holds")
+    _need(isinstance(max_own, int) and 0 <= max_own <= room, "max_own must be between 0 and what a row of block_tables holds")
     if out is not None:
-        _need(out.dtype == torch.bfloat16 and out.dim() == 2 and out.shape[0] >= T and out.shape[1] >= nh * D and out.stride(1) == 1,
+        _need(out.dtype == bf16 and out.dim() == 2 and out.shape[0] >= T and out.shape[1] >= nh * D and out.stride(1) == 1,
               "out bf16 [>= T, >= nh * D]")
     return B, kv8, max_own
 
@@ -412,7 +418,7 @@ def token_logprobs_check(logits, tokens, top_n, vocab):
     _need(0 < V <= logits.shape[1], "vocab must be between 1 and the width of logits")
     _need(tokens is None or (tokens.dtype == torch.int64 and tokens.dim() == 1 and tokens.numel() >= B and tokens.is_contiguous()),
           "tokens int64 [B]")
-    _need(0 <= top_n <= min(64, V), "top_n must be between 0 and min(64, vocab)")
+    _need(isinstance(top_n, int) and 0 <= top_n <= min(64, V), "top_n must be between 0 and min(64, vocab)")
     return B, V
 
 
