@@ -6,9 +6,11 @@
 //
 // Bound by memory: each logit is read and written once. A workgroup owns a run of CH tokens of a row; it walks the row's known tokens and
 // biases (from the caches: they are few beside the logits) and keeps what concerns its run in LDS - a counter a token, of 16 bits (two
-// in a word) up to 16383 known tokens and 32 beyond, with a bit for "seen" and one for "has a bias"; biases in a hash table. Then it
-// streams its run with 16-byte accesses, and only tokens whose counter is not zero cost more than a copy. Integer counts, and biases
-// summed in the order of the list: the result does not depend on the order in which threads run.
+// in a word) up to 32767 known tokens and 32 beyond, with a bit for "seen"; the run's biases as a list in their order. The logits are
+// asked for first and come meanwhile; then the run goes through with 16-byte accesses, and only tokens whose counter is not zero cost more
+// than a copy. Biased tokens are written once more at the end, by a thread each (found in the stream, by a table of them in LDS, 300
+// biases a row cost 256 x 131071 fp32 logits 27 us beside 48). Integer counts, and biases summed in the order of the list: the result does
+// not depend on the order in which threads run.
 #include "common.h"
 
 #include <type_traits>
@@ -35,7 +37,7 @@ struct LogitRules {
   const unsigned* mask;
   int64_t ldm;
   const int* mask_rows;
-  int masks, V, table, wide;  // wide: ids of 64 bits
+  int masks, V, wide;  // wide: ids of 64 bits
 };
 
 template <typename T>
@@ -76,20 +78,17 @@ __device__ __forceinline__ void store1(T* p, float v) {
   else *p = v;
 }
 
-__device__ __forceinline__ unsigned hash_of(int t) { return (unsigned)t * 2654435761u; }
-
 // W: 16-bit counters, else 32. VEC: rows of both sides on 16 bytes.
 template <typename TI, typename TO, bool W16, bool VEC>
 __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRules a, int CH) {
   extern __shared__ __attribute__((aligned(16))) unsigned lds[];
   const int b = blockIdx.y, lo = blockIdx.x * CH, n = min(CH, a.V - lo);
-  constexpr unsigned kSeen = W16 ? 0x8000u : 0x80000000u, kBias = W16 ? 0x4000u : 0x40000000u, kCount = kBias - 1;
+  constexpr unsigned kSeen = W16 ? 0x8000u : 0x80000000u, kCount = kSeen - 1;
   unsigned* cnt = lds;
   const int words = W16 ? CH / 2 : CH;
-  int* key = (int*)(lds + words);  // hash table of biased tokens: token, first entry, sum
-  int* first = key + a.table;
-  float* sum = (float*)(first + a.table);
-  __shared__ int twice;
+  int* list_t = (int*)(lds + words);  // the run's biases: tokens, values
+  float* list_v = (float*)(list_t + a.biases);
+  __shared__ int waves[2][kThreads / 64];
   const TI* x = (const TI*)a.x + (int64_t)b * a.ldx + lo;
   TO* y = (TO*)a.y + (int64_t)b * a.ldy + lo;
 
@@ -97,7 +96,19 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
   const int len = a.lens && (a.rep || a.pres || a.freq) ? min(max(a.lens[b], 0), a.most) : 0;
   const int mrow = a.mask ? (a.mask_rows ? a.mask_rows[b] : b) : -1;
   const unsigned* mask = mrow >= 0 && mrow < a.masks ? a.mask + (int64_t)mrow * a.ldm : nullptr;
-  const bool marks = len > 0 || a.biases > 0;
+  const bool marks = len > 0;
+  // (each thread's one or two entries; they are placed below)
+  static_assert(kMostBiases == 2 * kThreads, "two entries a thread");
+  int bt[2] = {-1, -1};
+  float bv[2] = {0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = k * kThreads + threadIdx.x;
+    if (i < a.biases) {
+      bt[k] = a.bias_ids[(int64_t)b * a.ldb + i];
+      bv[k] = a.bias[(int64_t)b * a.ldb + i];
+    }
+  }
   // the logits themselves are asked for first: they come while the known tokens are walked
   float v[VEC ? kPacks : 1][8];
   const int n8 = n & ~7;
@@ -116,11 +127,6 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
   };
   if (marks) {
     for (int i = threadIdx.x * 4; i < words; i += kThreads * 4) *reinterpret_cast<u32x4*>(cnt + i) = u32x4{0, 0, 0, 0};
-    for (int i = threadIdx.x; i < a.table; i += kThreads) {
-      key[i] = -1;
-      first[i] = INT_MAX;
-    }
-    if (threadIdx.x == 0) twice = 0;
     __syncthreads();
     const int prompt = a.prompts ? min(max(a.prompts[b], 0), len) : 0;
     for (int i0 = threadIdx.x; i0 < len; i0 += 4 * kThreads) {
@@ -139,58 +145,69 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
         else mark((int)t[k], kSeen, false);
       }
     }
-    // each biased token of the run gets a place in the table; the first of its entries owns it
-    const int* bi = a.bias_ids + (int64_t)b * a.ldb;
-    const float* bv = a.bias + (int64_t)b * a.ldb;
-    auto place = [&](int t) {
-      unsigned h = hash_of(t) & (a.table - 1);
-      while (true) {
-        const int was = atomicCAS(key + h, -1, t);
-        if (was == -1 || was == t) return h;
-        h = (h + 1) & (a.table - 1);
-      }
-    };
-    for (int i = threadIdx.x; i < a.biases; i += kThreads) {
-      const int t = bi[i] - lo;
-      if (bi[i] < 0 || t < 0 || t >= n) continue;
-      if (atomicMin(first + place(t), i) != INT_MAX) twice = 1;
-      mark(t, kBias, false);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.biases; i += kThreads) {
-      const int t = bi[i] - lo;
-      if (bi[i] < 0 || t < 0 || t >= n) continue;
-      const unsigned h = place(t);
-      if (first[h] != i) continue;
-      float s = bv[i];
-      if (twice)
-        for (int j = i + 1; j < a.biases; ++j)
-          if (bi[j] == bi[i]) s += bv[j];
-      sum[h] = s;
-    }
     __syncthreads();
   }
-  auto bias_of = [&](int t) {
-    unsigned h = hash_of(t) & (a.table - 1);
-    while (key[h] != t) h = (h + 1) & (a.table - 1);
-    return sum[h];
-  };
-  auto rules = [&](float v, unsigned c, int t) {
+  auto rules = [&](float v, unsigned c) {
     const unsigned times = c & kCount;
     if (times || (c & kSeen)) v = v > 0.f ? v / r : v * r;
     if (times) v = __fsub_rn(__fsub_rn(v, __fmul_rn((float)times, f)), p);
-    if (c & kBias) v += bias_of(t);
     return v;
   };
+  auto counter = [&](int t) { return W16 ? (cnt[t >> 1] >> (t & 1 ? 16 : 0)) & 0xffffu : cnt[t]; };
+  auto masked = [&](int t) { return mask && !(mask[(lo + t) >> 5] >> ((lo + t) & 31) & 1); };
   auto one = [&](int t) {
     float v = load1(x + t);
     if (marks) {
-      const unsigned c = W16 ? (cnt[t >> 1] >> (t & 1 ? 16 : 0)) & 0xffffu : cnt[t];
-      if (c) v = rules(v, c, t);
+      const unsigned c = counter(t);
+      if (c) v = rules(v, c);
     }
-    if (mask && !(mask[(lo + t) >> 5] >> ((lo + t) & 31) & 1)) v = -INFINITY;
-    store1(y + t, v);
+    store1(y + t, masked(t) ? -INFINITY : v);
   };
+  // the run's biases as a list in their order; each entry's token is the first entry's, whose thread sums it and writes the token at
+  // the end, from the logit that it takes before any is overwritten
+  int mine[2] = {-1, -1}, found = 0;
+  float was[2], add[2];
+  if (a.biases > 0) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    unsigned long long in[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      in[k] = __ballot(bt[k] >= lo && bt[k] < lo + n);
+      if (lane == 0) waves[k][w] = __popcll(in[k]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      int at = found + __popcll(in[k] & ((1ull << lane) - 1));
+      for (int i = 0; i < kThreads / 64; ++i) {
+        at += i < w ? waves[k][i] : 0;
+        found += waves[k][i];
+      }
+      if (in[k] >> lane & 1) {
+        list_t[at] = bt[k] - lo;
+        list_v[at] = bv[k];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = k * kThreads + threadIdx.x;
+      if (e >= found) continue;
+      const int t = list_t[e];
+      was[k] = load1(x + t);
+      float sum = 0.f;
+      bool first = true, any = false;
+      for (int j = 0; j < found; ++j) {
+        if (list_t[j] != t) continue;
+        if (j < e) first = false;
+        sum = any ? sum + list_v[j] : list_v[j];
+        any = true;
+      }
+      add[k] = sum;
+      if (first) mine[k] = t;
+    }
+    __syncthreads();
+  }
   if constexpr (!VEC) {
     for (int t = threadIdx.x; t < n; t += kThreads) one(t);
   } else {
@@ -222,7 +239,7 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
         if (any) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (c[i]) v[k][i] = rules(v[k][i], c[i], t + i);
+            if (c[i]) v[k][i] = rules(v[k][i], c[i]);
         }
       }
 #pragma unroll
@@ -230,6 +247,19 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
       store8(y + t, v[k]);
     }
     for (int t = n8 + threadIdx.x; t < n; t += kThreads) one(t);
+  }
+  if (a.biases > 0) {
+    __syncthreads();  // (what was written above is there)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (mine[k] < 0) continue;
+      float v = was[k];
+      if (marks) {
+        const unsigned c = counter(mine[k]);
+        if (c) v = rules(v, c);
+      }
+      store1(y + mine[k], masked(mine[k]) ? -INFINITY : v + add[k]);
+    }
   }
 }
 
@@ -239,7 +269,7 @@ void launch_rules(const LogitRules& a, int B, bool w16, hipStream_t st) {
   int CH = 1024;
   while (CH < (w16 ? kMostRun : kMostRun / 2) && (int64_t)B * ((a.V + CH - 1) / CH) > 1024) CH *= 2;
   const dim3 grid((a.V + CH - 1) / CH, B);
-  const size_t lds = (size_t)(w16 ? CH * 2 : CH * 4) + (size_t)a.table * 12;
+  const size_t lds = (size_t)(w16 ? CH * 2 : CH * 4) + (size_t)a.biases * 8;
 #define LR(W_, V_) adjust_logits_kernel<TI, TO, W_, V_><<<grid, kThreads, lds, st>>>(a, CH)
   if (w16) {
     if (vec) LR(true, true);
@@ -283,10 +313,7 @@ void launch_adjust_logits(const void* x, int64_t ldx, bool x32, void* y, int64_t
   a.masks = masks;
   a.V = V;
   a.wide = ids64;
-  a.table = 0;
-  if (a.biases)  // a power of two, at most half full
-    for (a.table = 4; a.table < 2 * a.biases;) a.table *= 2;
-  const bool w16 = most < 0x4000;
+  const bool w16 = most < 0x8000;
   if (x32) launch_rules<float, float>(a, B, w16, st);
   else if (y32) launch_rules<bf16_t, float>(a, B, w16, st);
   else launch_rules<bf16_t, bf16_t>(a, B, w16, st);

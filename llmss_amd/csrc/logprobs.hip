@@ -6,7 +6,7 @@
 // of exponentials, how many of its tokens are ahead of the given one, and its own n likeliest in order; a second launch joins a row's
 // runs. The n likeliest of a run: a number that at least n tokens reach is found from the lanes' own maxima (a binary search over the
 // upper bits of an order-preserving key, by ballots), and the few tokens that reach it are ranked by counting. Keys carry the token behind
-// the value, so no two are equal: where a run of equal logits has more than the short list takes, the search goes on over all bits. A NaN counts as no candidate, and makes its row's
+// the value, so no two are equal: where a run of equal logits has more than the list takes, the search goes on over all bits. A NaN counts as no candidate, and makes its row's
 // log-probabilities NaN; a row of nothing but -inf has log-probabilities of -inf.
 #include "common.h"
 
@@ -34,9 +34,6 @@ __device__ __forceinline__ float at(const T* p) {
   else return *p;
 }
 
-// Lists of a run's likeliest hold this many keys; a run of ties that has more takes the exact way, whose list is at most kNT x 8 PACKS long.
-constexpr int kShort = 512;
-
 // NT threads, PACKS x 8 tokens a thread. Partial results of run c of row b: part[b][c] = (m, s, ahead, -), top[b][c][n] keys.
 template <typename T, int NT, int PACKS, bool VEC>
 __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ tokens, int V,
@@ -46,8 +43,7 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const T* row = logits + (int64_t)b * ld;
   __shared__ float red[NW], reds[NW], line[NW];
-  __shared__ int redn[NW], found;
-  __shared__ u64 low[NW];
+  __shared__ int redn[NW], redc[NW], found;
   extern __shared__ __attribute__((aligned(16))) u64 list[];  // cap keys
   const int64_t tok = tokens ? tokens[b] : -1;
   float x[PACKS][8];
@@ -100,20 +96,32 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
     redn[w] = ahead;
   }
   if (n > 0) {
-    // a value that n of the wave's lanes reach with their best (-inf: fewer do), to the upper 16 bits of its key
+    // a value that so many of the wave's lanes reach with their best (-inf: fewer do), to the upper 16 bits of its key
     const unsigned best = (unsigned)(key_of(m, 0) >> 32);
-    unsigned reach = 0;
+    auto reached_by = [&](int lanes) {
+      unsigned reach = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
-      const unsigned want = reach | 1u << bit;
-      if (__popcll(__ballot(best >= want)) >= n) reach = want;
-    }
-    if (lane == 0) line[w] = reach <= 0x007fffffu ? -INFINITY : value_of((u64)reach << 32);
+      for (int bit = 31; bit >= 16; --bit) {
+        const unsigned want = reach | 1u << bit;
+        if (__popcll(__ballot(best >= want)) >= lanes) reach = want;
+      }
+      return reach <= 0x007fffffu ? -INFINITY : value_of((u64)reach << 32);
+    };
+    const float part_of = reached_by((n + NW - 1) / NW);  // each wave's share of n: all reach the least of them
+    if (lane == 0) line[w] = part_of;
     if (threadIdx.x == 0) found = 0;
     __syncthreads();
     float L = line[0];
 #pragma unroll
-    for (int i = 1; i < NW; ++i) L = fmaxf(L, line[i]);
+    for (int i = 1; i < NW; ++i) L = fminf(L, line[i]);
+    if (L == -INFINITY) {  // (a row's last run: waves without tokens) n of one wave
+      __syncthreads();
+      const float all_of = reached_by(n);
+      if (lane == 0) line[w] = all_of;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NW; ++i) L = fmaxf(L, line[i]);
+    }
     if (m >= L) {  // (a thread without a token has -inf)
 #pragma unroll
       for (int k = 0; k < PACKS; ++k)
@@ -130,8 +138,9 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
   __syncthreads();
   if (n > 0) {
     int have = found;
-    if (have > kShort) {  // (ties, or a run with few numbers: the same in every thread)
-      // the exact way: keys that hold the token too are never equal, so at most n lanes of a wave reach the line
+    if (have > cap) {  // (ties, or a run with few numbers: the same in every thread)
+      // the exact way: keys that hold the token too are never equal, so n threads and no more reach the line with their best, or all
+      // that have a token where those are fewer
       u64 best = 0;
 #pragma unroll
       for (int k = 0; k < PACKS; ++k)
@@ -141,18 +150,20 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
           const u64 q = t < V ? key_of(x[k][i], t) : 0ull;
           best = q > best ? q : best;
         }
-      u64 reach = 0;
+      u64 l = 0;
 #pragma unroll 1
       for (int bit = 63; bit >= 0; --bit) {
-        const u64 want = reach | 1ull << bit;
-        if (__popcll(__ballot(best >= want)) >= n) reach = want;
-      }
-      if (lane == 0) low[w] = reach;
-      __syncthreads();
-      if (threadIdx.x == 0) found = 0;
-      u64 l = low[0];
+        const u64 want = l | 1ull << bit;
+        const int mine = __popcll(__ballot(best >= want));
+        __syncthreads();  // (the counts of the bit before are read)
+        if (lane == 0) redc[w] = mine;
+        __syncthreads();
+        int all = 0;
 #pragma unroll
-      for (int i = 1; i < NW; ++i) l = low[i] > l ? low[i] : l;
+        for (int i = 0; i < NW; ++i) all += redc[i];
+        if (all >= n) l = want;
+      }
+      if (threadIdx.x == 0) found = 0;
       if (l == 0) l = 1;
       __syncthreads();
       if (best >= l) {
@@ -172,6 +183,7 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
     for (int i = threadIdx.x; i < have; i += NT) {
       const u64 q = list[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < have; ++j) rank += list[j] > q;
       if (rank < n) mine_top[rank] = q;
     }
@@ -286,6 +298,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
   for (int i = threadIdx.x; i < have; i += 256) {
     const u64 q = kept[i];
     int place = 0;
+#pragma unroll 8
     for (int c = 0; c < have; ++c) place += kept[c] > q;
     if (place < n) {
       top_ids[(int64_t)b * n + place] = (int)~(unsigned)q;
@@ -296,14 +309,13 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
 
 constexpr int kNT = 256;
 
-// 8-token packs of a thread: four, or one while those would fill the chip less than twice; two where the lists of the likeliest grow.
+// 8-token packs of a thread: four, or one while those would fill the chip less than twice and n is small against a run.
 int packs_of(int B, int V, int n) {
-  if (n > 32) return 2;
-  return V > (1 << 18) || (int64_t)B * ((V + 4 * 8 * kNT - 1) / (4 * 8 * kNT)) >= 512 ? 4 : 1;
+  return n > 20 || V > (1 << 18) || (int64_t)B * ((V + 4 * 8 * kNT - 1) / (4 * 8 * kNT)) >= 512 ? 4 : 1;
 }
 
-// Keys that a run's list holds: what the exact way may need, at most n threads of each wave.
-int list_of(int n, int packs) { return n == 0 ? 0 : std::max(kShort, std::min(4 * n, kNT) * packs * 8); }
+// Keys that a run's list holds: several times what is found as a rule, and what the exact way may need.
+int list_of(int n, int packs) { return n == 0 ? 0 : std::max(512, n * packs * 8); }
 
 }  // namespace
 
@@ -330,9 +342,6 @@ void launch_logprobs(const void* logits, int64_t ld, bool fp32, const void* toke
     if (packs == 4) {                                                                                                   \
       if (vec) LK(T_, 4, true);                                                                                         \
       else LK(T_, 4, false);                                                                                            \
-    } else if (packs == 2) {                                                                                            \
-      if (vec) LK(T_, 2, true);                                                                                         \
-      else LK(T_, 2, false);                                                                                            \
     } else {                                                                                                            \
       if (vec) LK(T_, 1, true);                                                                                         \
       else LK(T_, 1, false);                                                                                            \

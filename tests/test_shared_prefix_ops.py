@@ -372,8 +372,8 @@ def test_rules_pass_on_what_is_not_finite(dev):
 
 @pytest.mark.gpu
 def test_rules_of_long_histories():
-    """Counters of 16 bits up to 16383 known tokens, of 32 beyond; one token that was said each time."""
-    for known in (16383, 16384, 40000):
+    """Counters of 16 bits up to 32767 known tokens, of 32 beyond; one token that was said each time."""
+    for known in (16383, 16384, 32767, 32768, 40000):
         x = torch.randn(2, 3000, device="cuda")
         ids = torch.randint(0, 3000, (2, known), device="cuda")
         ids[1] = 17
@@ -486,7 +486,7 @@ def test_the_likeliest_of_sorted_rows():
     V = 40001
     up = torch.arange(V, dtype=torch.float32) * 1e-3
     x = torch.stack([up, up.flip(0), (torch.arange(V) % 2).float(), torch.zeros(V)]).cuda()
-    for n in (1, 20, 32, 33, 64):
+    for n in (1, 4, 5, 20, 32, 33, 64):
         _, _, ids, _ = ops.token_logprobs(x, None, n)
         assert torch.equal(ids, torch.sort(x, dim=-1, descending=True, stable=True)[1][:, :n])
 
