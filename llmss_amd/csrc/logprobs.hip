@@ -34,12 +34,12 @@ __device__ __forceinline__ float at(const T* p) {
   else return *p;
 }
 
-// NT threads, PACKS x 8 tokens a thread. Partial results of run c of row b: part[b][c] = (m, s, ahead, -), top[b][c][n] keys.
+// NT threads, up to PACKS x 8 tokens a thread, len a run. Partial results of run c of row b: part[b][c] = (m, s, ahead, -), top[b][c][n] keys.
 template <typename T, int NT, int PACKS, bool VEC>
 __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ tokens, int V,
-                                                           int n, int cap, float* __restrict__ part, u64* __restrict__ top) {
-  constexpr int NW = NT / 64, RUN = NT * PACKS * 8;
-  const int b = blockIdx.y, c = blockIdx.x, runs = gridDim.x, lo = c * RUN;
+                                                           int n, int len, int cap, float* __restrict__ part, u64* __restrict__ top) {
+  constexpr int NW = NT / 64;
+  const int b = blockIdx.y, c = blockIdx.x, runs = gridDim.x, lo = c * len, end = min(V, lo + len);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const T* row = logits + (int64_t)b * ld;
   __shared__ float red[NW], reds[NW], line[NW];
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
 #pragma unroll
   for (int k = 0; k < PACKS; ++k) {
     const int t = lo + (k * NT + threadIdx.x) * 8;
-    if (VEC && t + 8 <= V) {
+    if (VEC && t + 8 <= end) {
       if constexpr (sizeof(T) == 2) {
         const u16x8 v = *reinterpret_cast<const u16x8*>(row + t);
 #pragma unroll
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[k][i] = t + i < V ? at(row + t + i) : -INFINITY;
+      for (int i = 0; i < 8; ++i) x[k][i] = t + i < end ? at(row + t + i) : -INFINITY;
     }
   }
   const bool given = tok >= 0 && tok < V;
@@ -107,28 +107,23 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
       }
       return reach <= 0x007fffffu ? -INFINITY : value_of((u64)reach << 32);
     };
-    const float part_of = reached_by((n + NW - 1) / NW);  // each wave's share of n: all reach the least of them
+    // each wave's share of n, by the threads of it that have tokens: all of a share reach the least of the waves' values
+    const int holders = min(NT, (end - lo + 7) / 8), held = min(max(holders - w * 64, 0), 64);
+    const float part_of = held ? reached_by((n * held + holders - 1) / holders) : INFINITY;
     if (lane == 0) line[w] = part_of;
     if (threadIdx.x == 0) found = 0;
     __syncthreads();
     float L = line[0];
 #pragma unroll
     for (int i = 1; i < NW; ++i) L = fminf(L, line[i]);
-    if (L == -INFINITY) {  // (a row's last run: waves without tokens) n of one wave
-      __syncthreads();
-      const float all_of = reached_by(n);
-      if (lane == 0) line[w] = all_of;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NW; ++i) L = fmaxf(L, line[i]);
-    }
+    if (holders < n) L = -INFINITY;
     if (m >= L) {  // (a thread without a token has -inf)
 #pragma unroll
       for (int k = 0; k < PACKS; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int t = lo + (k * NT + threadIdx.x) * 8 + i;
-          if (x[k][i] >= L && t < V) {
+          if (x[k][i] >= L && t < end) {
             const int p = atomicAdd(&found, 1);
             if (p < cap) list[p] = key_of(x[k][i], t);
           }
@@ -147,7 +142,7 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int t = lo + (k * NT + threadIdx.x) * 8 + i;
-          const u64 q = t < V ? key_of(x[k][i], t) : 0ull;
+          const u64 q = t < end ? key_of(x[k][i], t) : 0ull;
           best = q > best ? q : best;
         }
       u64 l = 0;
@@ -172,7 +167,7 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int t = lo + (k * NT + threadIdx.x) * 8 + i;
-            const u64 q = t < V ? key_of(x[k][i], t) : 0ull;
+            const u64 q = t < end ? key_of(x[k][i], t) : 0ull;
             if (q >= l) list[atomicAdd(&found, 1)] = q;
           }
       }
@@ -324,18 +319,20 @@ int logprobs_runs(int B, int V, int n) {
   return (V + run - 1) / run;
 }
 
+
 void launch_logprobs(const void* logits, int64_t ld, bool fp32, const void* tokens, int B, int V, int n, void* part, void* top, void* lp,
                      void* rank, void* top_ids, void* top_lp, hipStream_t st) {
   if (B == 0) return;
   if (B > 65535) throw std::runtime_error("token_logprobs: at most 65535 rows");
   if (n < 0 || n > kMostTop || n > V) throw std::runtime_error("token_logprobs: top_n must be between 0 and min(64, vocab)");
   const int packs = packs_of(B, V, n), runs = logprobs_runs(B, V, n);
+  const int len = ((V + runs - 1) / runs + 7) / 8 * 8;  // (runs of a row as long as each other: a short last one has no better line)
   const size_t join = (size_t)runs * n * 8;
   if (V >= 1 << 24 || join > 30 * 1024) throw std::runtime_error("token_logprobs: vocabulary too large");
   const bool vec = (uintptr_t)logits % 16 == 0 && ld * (fp32 ? 4 : 2) % 16 == 0;
   const dim3 grid(runs, B);
 #define LK(T_, P_, V_)                                                                                                  \
-  logprobs_runs_kernel<T_, kNT, P_, V_><<<grid, kNT, (size_t)list_of(n, P_) * 8, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, list_of(n, P_), \
+  logprobs_runs_kernel<T_, kNT, P_, V_><<<grid, kNT, (size_t)list_of(n, P_) * 8, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, len, list_of(n, P_), \
                                                                                 (float*)part, (u64*)top)
 #define LP(T_)                                                                                                          \
   do {                                                                                                                  \
