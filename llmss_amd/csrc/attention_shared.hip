@@ -156,6 +156,20 @@ __device__ __forceinline__ int wave_max(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
+// The order of a block's reads of LDS and matrix instructions: AHEAD reads first, then after every M matrix instructions R reads more,
+// until N are made. Left alone the compiler reads one fragment ahead, and every product waits most of a read's time.
+template <int N, int AHEAD, int R, int M>
+__device__ __forceinline__ void read_ahead() {
+  constexpr int kRead = 0x100, kMfma = 0x8;
+  __builtin_amdgcn_sched_group_barrier(kRead, AHEAD, 0);
+#pragma unroll
+  for (int i = AHEAD; i < N; i += R) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, M, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kMfma, AHEAD / R * M, 0);
+}
+
 // 16-byte chunk c of row r in an LDS image of unpadded rows: rows of 16 reads and of transposing reads fall on different banks.
 template <int D>
 __device__ __forceinline__ int swz(int c, int r) {
@@ -242,7 +256,7 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS],
 // O^T += V^T P^T. Where a tile that is masked for some slots holds values that are not finite, the products would give them to every
 // slot (0 times such a value is NaN): there the weights go through `own_lds` (16 slots of 16 KT keys, the wave's own) and each slot
 // takes the keys that it sees one after the other. Rare, so kept small.
-template <int D, int KT, int NS>
+template <int D, int KT, int NS, bool FEW>
 __device__ __forceinline__ void add_values(bool masked, const char* img, bf16_t* own_lds, const int (&lim)[NS], int g_, int li_,
                                            const s16x8 (&pf)[NS][KT / 2], f32x4 (&o)[NS][D / 16]) {
   if (masked) {
@@ -291,8 +305,9 @@ __device__ __forceinline__ void add_values(bool masked, const char* img, bf16_t*
       const s16x8 vf = v_fragment<D>(img, 32 * k, dt, g_, li_);
 #pragma unroll
       for (int n = 0; n < NS; ++n) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][k], o[n][dt], 0, 0, 0);
-      if (KT == 2 && NS == 1 && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (second form: no registers for more reads ahead)
+      if (FEW && dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (second form: no registers for more reads ahead)
     }
+  if constexpr (!FEW) read_ahead<KT / 2 * (D / 16) * 2, 8, 2, NS>();
 }
 
 // A softmax over several sets of keys from the sets' (m, l) and four of their outputs.
@@ -520,6 +535,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
 #pragma unroll
           for (int n = 0; n < NS; ++n) s[n][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt], qf[n][ks], s[n][kt], 0, 0, 0);
       }
+      read_ahead<KT * (D / 32), 6, 1, NS>();
       __builtin_amdgcn_sched_barrier(0);
       const float* vs = nullptr;
       if constexpr (KV8) {
@@ -539,7 +555,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
       for (int n = 0; n < NS; ++n) left[n] = MASK ? min(lim[n], it.stop) - kv0 : BKV;
       s16x8 pf[NS][KT / 2];
       soften<D, KT, NS, MASK>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
-      add_values<D, KT, NS>(MASK, sk + TILE, apart + w * 16 * BKV, left, g, li, pf, o);
+      add_values<D, KT, NS, false>(MASK, sk + TILE, apart + w * 16 * BKV, left, g, li, pf, o);
     };
     // tiles that every slot of the wave sees whole come first, in a loop without masks
     const int whole = min(max(0, (min(wave_lo, it.stop) - it.begin) / BKV), ntiles);
@@ -717,7 +733,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       const int left[1] = {min(lim[0], it.stop) - kv0};
       soften<D, KT, 1, true>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
       const int l = anew();
-      add_values<D, KT, 1>(kv0 + BK > min(lo, it.stop), img, apart + w * 16 * BK, left, l >> 4, l & 15, pf, o);
+      add_values<D, KT, 1, true>(kv0 + BK > min(lo, it.stop), img, apart + w * 16 * BK, left, l >> 4, l & 15, pf, o);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the place is read)
     }
   }
