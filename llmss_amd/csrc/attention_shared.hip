@@ -47,7 +47,7 @@ struct SharedAttn {
   bf16_t* out;
   int64_t out_stride;
   int parts, finish;  // partial results of a (row, head); whether the own parts' launch joins them itself
-  int64_t page_bytes;
+  unsigned page_bytes;
   int T, B, nh, nkv, G, bs, shift, pages, P, own_cap;  // shift: log2 of bs where it is a power of two
   int pre_items, pre_tiles, pre_split, pre_keys, pre_few;
   int own_tiles, own_split, own_keys, own_few;
@@ -94,17 +94,23 @@ struct Rows {
   const SharedAttn& a;
   const Item& it;
   int ids = 0;
+  // a page's first byte of this key head; one that the cache does not have counts as the first
   __device__ __forceinline__ int64_t start(int page) const {
     const unsigned p = (unsigned)page < (unsigned)a.pages ? (unsigned)page : 0u;
-    return (int64_t)p * a.page_bytes + (int64_t)it.kvh * a.bs * RB;
+    return (int64_t)((uint64_t)p * a.page_bytes) + (int64_t)it.kvh * a.bs * RB;
   }
+  __device__ __forceinline__ int base(int kv0, int run) const { return min(kv0 + 16 * run, (it.stop - 1) & ~15); }
   __device__ __forceinline__ void ask(int kv0) {  // (in front of other accesses to memory: else it is moved to where its answer is used)
     if constexpr (BY16) ids = it.table[min(kv0 + 16 * (int)(threadIdx.x % KT), it.stop - 1) >> a.shift];
   }
-  __device__ __forceinline__ int page(int run) const { return BY16 ? __builtin_amdgcn_readlane(ids, run) : 0; }
-  // row r < 16 of run `run` of a tile, whose page is pg (both the same in every lane); keys past the last stand for the last
-  __device__ __forceinline__ int base(int kv0, int run) const { return min(kv0 + 16 * run, (it.stop - 1) & ~15); }
-  __device__ __forceinline__ int64_t run_at(int pg, int kv0, int run) const { return start(pg) + (base(kv0, run) & (a.bs - 1)) * RB; }
+  // what was asked for: the bytes in front of each run of the tile, a run a lane
+  __device__ __forceinline__ int64_t asked(int kv0) const {
+    return BY16 ? start(ids) + (base(kv0, threadIdx.x % KT) & (a.bs - 1)) * RB : 0;
+  }
+  __device__ __forceinline__ int64_t of_run(int64_t runs, int run) const {
+    return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(runs >> 32), run) << 32 | (unsigned)__builtin_amdgcn_readlane((int)runs, run));
+  }
+  // row r < 16 of run `run` of a tile, the same run in every lane; keys past the last stand for the last
   __device__ __forceinline__ unsigned row_at(int kv0, int run, int r) const { return min(r, it.stop - 1 - base(kv0, run)) * RB; }
   __device__ __forceinline__ int64_t alone(int k) const {
     k = min(k, it.stop - 1);
@@ -112,8 +118,8 @@ struct Rows {
     return start(it.table[i]) + (k - i * a.bs) * RB;
   }
   template <typename V>
-  __device__ __forceinline__ V load(const void* cache, int pg, int kv0, int run, int r, unsigned more) const {
-    if constexpr (BY16) return *reinterpret_cast<const V*>((const char*)cache + run_at(pg, kv0, run) + (row_at(kv0, run, r) + more));
+  __device__ __forceinline__ V load(const void* cache, int64_t run_at, int kv0, int run, int r, unsigned more) const {
+    if constexpr (BY16) return *reinterpret_cast<const V*>((const char*)cache + run_at + (row_at(kv0, run, r) + more));
     else return *reinterpret_cast<const V*>((const char*)cache + alone(kv0 + 16 * run + r) + more);
   }
   // 16 bytes a lane from memory into LDS (lane l at `at` + 16 l, the same `at` in every lane). Through inline assembly, so that the compiler does not hold reads
@@ -121,9 +127,9 @@ struct Rows {
   __device__ __forceinline__ void to_lds(const char* p, unsigned off, unsigned at) const {  // (all of a run's rows: p the run's, off a lane's)
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory");
   }
-  __device__ __forceinline__ void to_lds(const void* cache, int pg, int kv0, int run, int r, unsigned more, unsigned at) const {
+  __device__ __forceinline__ void to_lds(const void* cache, int64_t run_at, int kv0, int run, int r, unsigned more, unsigned at) const {
     if constexpr (BY16) {
-      const char* p = (const char*)cache + run_at(pg, kv0, run);
+      const char* p = (const char*)cache + run_at;
       const unsigned off = row_at(kv0, run, r) + more;
       asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory");
     } else {
@@ -463,10 +469,11 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
       const int kv0 = it.begin + j * BKV;
       const unsigned sl = lds0 + (j & 1) * 2 * TILE;
       if constexpr (KV8) {
-        int pg[PIECES];
+        const int64_t runs = rows.asked(kv0);
+        int64_t pg[PIECES];
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)  // (16 rows of 4, 8 or 16 pieces: a wave's rows lie within one run of 16)
-          pg[i] = rows.page(__builtin_amdgcn_readfirstlane((threadIdx.x + i * 256) / D));
+          pg[i] = rows.of_run(runs, __builtin_amdgcn_readfirstlane((threadIdx.x + i * 256) / D));
         rows.ask(kv0 + BKV);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
@@ -477,15 +484,16 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
         if (threadIdx.x < 2 * BKV)
           sc = *reinterpret_cast<const float*>((const char*)(threadIdx.x < BKV ? a.kc : a.vc) + rows.alone(kv0 + threadIdx.x % BKV) + D);
       } else {
-        int pg[LPW];
+        const int64_t runs = rows.asked(kv0);
+        int64_t pg[LPW];
 #pragma unroll
-        for (int i = 0; i < LPW; ++i) pg[i] = rows.page((i * 4 + w) * RPI / 16);
+        for (int i = 0; i < LPW; ++i) pg[i] = rows.of_run(runs, (i * 4 + w) * RPI / 16);
         rows.ask(kv0 + BKV);
         if (BY16 && kv0 + BKV <= it.stop) {  // (a lane's row in its run and its chunk are the same for every instruction but for 8 rows)
 #pragma unroll
           for (int i = 0; i < LPW; ++i) {
             const int inst = i * 4 + w;
-            const int64_t at = rows.run_at(pg[i], kv0, inst * RPI / 16) + (D == 256 ? (i & 1) * 8 * 2 * D : 0);
+            const int64_t at = pg[i] + (D == 256 ? (i & 1) * 8 * 2 * D : 0);
             rows.to_lds((const char*)a.kc + at, lane_off, sl + inst * 1024);
             rows.to_lds((const char*)a.vc + at, lane_off, sl + TILE + inst * 1024);
           }
@@ -650,7 +658,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
     constexpr int RPI = 64 / CH, INS = BK / RPI, PIECES = BK * (D / 16) / 64;
     u32x4 v8[KV8 ? PIECES : 1];
     float sc = 0.f;
-    auto keys = [&](int kv0, const int (&pg)[KT]) {
+    auto keys = [&](int kv0, const int64_t (&pg)[KT]) {
       const int l = anew(), li = l & 15, g = l >> 4;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
@@ -664,7 +672,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       }
       if constexpr (KV8) sc = *reinterpret_cast<const float*>((const char*)(lane < BK ? a.kc : a.vc) + rows.alone(kv0 + lane % BK) + D);
     };
-    auto values = [&](int kv0, const int (&pg)[KT]) {
+    auto values = [&](int kv0, const int64_t (&pg)[KT]) {
       const int lane = anew();
       if constexpr (KV8) {
 #pragma unroll
@@ -681,10 +689,11 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
         }
       }
     };
-    int pg[KT];
+    int64_t pg[KT];
     auto pages = [&](int kv0) {  // those asked for, and what lies a turn behind them is asked for
+      const int64_t runs = rows.asked(kv0);
 #pragma unroll
-      for (int i = 0; i < KT; ++i) pg[i] = rows.page(i);
+      for (int i = 0; i < KT; ++i) pg[i] = rows.of_run(runs, i);
       rows.ask(kv0 + step);
     };
 #pragma unroll 1
@@ -933,7 +942,9 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
   a.G = nh / nkv;
   a.bs = bs;
   a.shift = __builtin_ctz(bs);
-  a.page_bytes = (int64_t)nkv * bs * (kv8 ? D + kTail : 2 * D);
+  const int64_t page_bytes = (int64_t)nkv * bs * (kv8 ? D + kTail : 2 * D);
+  if (page_bytes > INT_MAX) throw std::runtime_error("attn_shared: pages of 2 GiB and more");
+  a.page_bytes = (unsigned)page_bytes;
   a.pages = pages;
   a.P = P;
   a.own_cap = (int)std::min<int64_t>((int64_t)bt_width * bs, INT_MAX / 2);
