@@ -107,6 +107,11 @@ struct Rows {
   __device__ __forceinline__ int64_t asked(int kv0) const {
     return BY16 ? start(ids) + (base(kv0, threadIdx.x % KT) & (a.bs - 1)) * RB : 0;
   }
+  // the bytes in front of a lane's own row of the tile
+  __device__ __forceinline__ int64_t own_row(int64_t runs, int kv0, int row) const {
+    if constexpr (BY16) return __shfl(runs, row >> 4, 64) + min(row & 15, it.stop - 1 - base(kv0, row >> 4)) * RB;
+    else return alone(kv0 + row);
+  }
   __device__ __forceinline__ int64_t of_run(int64_t runs, int run) const {
     return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(runs >> 32), run) << 32 | (unsigned)__builtin_amdgcn_readlane((int)runs, run));
   }
@@ -469,7 +474,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
       const int kv0 = it.begin + j * BKV;
       const unsigned sl = lds0 + (j & 1) * 2 * TILE;
       if constexpr (KV8) {
-        const int64_t runs = rows.asked(kv0);
+        const int64_t runs = rows.asked(kv0), at = rows.own_row(runs, kv0, threadIdx.x % BKV);
         int64_t pg[PIECES];
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)  // (16 rows of 4, 8 or 16 pieces: a wave's rows lie within one run of 16)
@@ -482,7 +487,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
           v8[i] = rows.template load<u32x4>(a.vc, pg[i], kv0, run, r & 15, (c % (D / 16)) * 16);
         }
         if (threadIdx.x < 2 * BKV)
-          sc = *reinterpret_cast<const float*>((const char*)(threadIdx.x < BKV ? a.kc : a.vc) + rows.alone(kv0 + threadIdx.x % BKV) + D);
+          sc = *reinterpret_cast<const float*>((const char*)(threadIdx.x < BKV ? a.kc : a.vc) + at + D);
       } else {
         const int64_t runs = rows.asked(kv0);
         int64_t pg[LPW];
@@ -658,6 +663,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
     constexpr int RPI = 64 / CH, INS = BK / RPI, PIECES = BK * (D / 16) / 64;
     u32x4 v8[KV8 ? PIECES : 1];
     float sc = 0.f;
+    int64_t scale_at = 0;
     auto keys = [&](int kv0, const int64_t (&pg)[KT]) {
       const int l = anew(), li = l & 15, g = l >> 4;
 #pragma unroll
@@ -670,7 +676,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
           for (int ks = 0; ks < D / 32; ++ks) kf[kt][ks] = rows.template load<s16x8>(a.kc, pg[kt], kv0, kt, li, 64 * ks + 16 * g);
         }
       }
-      if constexpr (KV8) sc = *reinterpret_cast<const float*>((const char*)(lane < BK ? a.kc : a.vc) + rows.alone(kv0 + lane % BK) + D);
+      if constexpr (KV8) sc = *reinterpret_cast<const float*>((const char*)(lane < BK ? a.kc : a.vc) + scale_at);
     };
     auto values = [&](int kv0, const int64_t (&pg)[KT]) {
       const int lane = anew();
@@ -692,6 +698,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
     int64_t pg[KT];
     auto pages = [&](int kv0) {  // those asked for, and what lies a turn behind them is asked for
       const int64_t runs = rows.asked(kv0);
+      if constexpr (KV8) scale_at = rows.own_row(runs, kv0, threadIdx.x % BK) + D;
 #pragma unroll
       for (int i = 0; i < KT; ++i) pg[i] = rows.of_run(runs, i);
       rows.ask(kv0 + step);
