@@ -202,8 +202,9 @@ __device__ __forceinline__ s16x8 v_fragment(const char* img, int r32, int dt, in
 // Scores of 16 KT keys and NS groups of slots become weights: the running maximum of a slot moves only where its own has grown by
 // more than 8 (weights stay below 2^8), so most tiles exchange nothing between lanes and rescale nothing. Weights are rounded to
 // bf16 for the second product (half a step of 2^-8, as any bf16 operand); their sum is taken of the rounded ones, by a product with
-// ones, so that they add up to 1 as they are used. lim: keys [.., lim) are seen, counted from the tile's first.
-template <int D, int KT, int NS, bool MASK>
+// ones, so that they add up to 1 as they are used. fp8 rows: a weight times its row's scale is what is rounded, so the sum is of the
+// weights themselves, by lane (the lanes of a slot meet at the end). lim: keys [.., lim) are seen, counted from the tile's first.
+template <int D, int KT, int NS, bool MASK, bool KV8>
 __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS], float scale_log2, int g, float (&m)[NS],
                                        f32x4 (&lsum)[NS], f32x4 (&o)[NS][D / 16], s16x8 (&pf)[NS][KT / 2], const float* vscale) {
   float mx[NS];
@@ -241,25 +242,26 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS],
   for (int n = 0; n < NS; ++n) {
     const float nm = -m[n];
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+    for (int kt = 0; kt < KT; ++kt) {
+      f32x4 v;
+      if constexpr (KV8) v = *reinterpret_cast<const f32x4*>(vscale + kt * 16 + 4 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[n][kt][i] = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i], scale_log2, nm));
-        pf[n][kt >> 1][(kt & 1) * 4 + i] = (short)f2bf(s[n][kt][i]);
-      }
-#pragma unroll
-    for (int k = 0; k < KT / 2; ++k) lsum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[n][k], lsum[n], 0, 0, 0);
-    if (vscale) {  // (fp8 rows: a weight times its row's scale, rounded once for the product and once for the sum)
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(vscale + kt * 16 + 4 * g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const short x = (short)f2bf(s[n][kt][i] * v[i]);
-          // (a key that is not seen: its scale may be anything)
-          pf[n][kt >> 1][(kt & 1) * 4 + i] = !MASK || s[n][kt][i] != 0.f ? x : (short)0;
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i], scale_log2, nm));
+        short w;
+        if constexpr (KV8) {
+          lsum[n][i] += p;
+          w = (short)f2bf(p * v[i]);
+          if (MASK && p == 0.f) w = 0;  // (a key that is not seen: its scale may be anything)
+        } else {
+          w = (short)f2bf(p);
         }
+        pf[n][kt >> 1][(kt & 1) * 4 + i] = w;
       }
+    }
+    if constexpr (!KV8) {
+#pragma unroll
+      for (int k = 0; k < KT / 2; ++k) lsum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[n][k], lsum[n], 0, 0, 0);
     }
   }
 }
@@ -386,6 +388,15 @@ __device__ __forceinline__ void add_parts(const float* ml, const float* x, int f
     for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[dt][e] = o[dt][e] * f + w[dt][e] * h;
+  }
+}
+
+// The sum of a slot's weights, in all four places, where it is kept by lane.
+template <bool KV8>
+__device__ __forceinline__ void meet(f32x4& lsum) {
+  if constexpr (KV8) {
+    const float l = xor32_sum(xor16_sum((lsum[0] + lsum[1]) + (lsum[2] + lsum[3])));
+    lsum = f32x4{l, l, l, l};
   }
 }
 
@@ -567,7 +578,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
 #pragma unroll
       for (int n = 0; n < NS; ++n) left[n] = MASK ? min(lim[n], it.stop) - kv0 : BKV;
       s16x8 pf[NS][KT / 2];
-      soften<D, KT, NS, MASK>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
+      soften<D, KT, NS, MASK, KV8>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
       add_values<D, KT, NS, false>(MASK, sk + TILE, apart + w * 16 * BKV, left, g, li, pf, o);
     };
     // tiles that every slot of the wave sees whole come first, in a loop without masks
@@ -604,6 +615,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
   }
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
+    meet<KV8>(lsum[n]);
     const int l = anew(), slot = it.first + (w * NS + n) * 16 + (l & 15);
     if (slot < it.slots) leave<D>(a, it, slot, l >> 4, o[n], m[n], lsum[n][0]);
   }
@@ -747,12 +759,13 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       const float* vs = KV8 ? fac + BK : nullptr;
       s16x8 pf[1][1];
       const int left[1] = {min(lim[0], it.stop) - kv0};
-      soften<D, KT, 1, true>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
+      soften<D, KT, 1, true, KV8>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
       const int l = anew();
       add_values<D, KT, 1, true>(kv0 + BK > min(lo, it.stop), img, apart + w * 16 * BK, left, l >> 4, l & 15, pf, o);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the place is read)
     }
   }
+  meet<KV8>(lsum[0]);
   const bool finish = it.own && a.finish;
   if (finish) {  // the own part is one workgroup's: the prefix's parts, left by the launch before, join it here, every fourth a wave
     const int l = anew(), slot = it.first + (l & 15), g = l >> 4;
