@@ -26,12 +26,13 @@
 // fp8 cache rows: e4m3 numbers are exact in bf16, a row's scale multiplies its score and its weight.
 #include "common.h"
 
+#include <cfloat>
 #include <type_traits>
 
 namespace {
 
 constexpr float kLog2eS = 1.4426950408889634f;
-constexpr float kFloor = -1.0e30f;  // a maximum before any key was seen
+constexpr float kFloor = -FLT_MAX;  // a maximum before any key was seen
 constexpr int kTail = 16;           // bytes behind the numbers of an fp8 cache row, the first four its scale
 
 struct SharedAttn {
@@ -335,21 +336,21 @@ struct Joined {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = o[e] * f + x[e] * h;
   }
-  // parts that lie one after the other, N asked for at a time
+  // parts first, first + step, .. < n, N asked for at a time
   template <int D, int N>
-  __device__ __forceinline__ void add_parts(const float* ml, const float* x, int n) {
-    for (int p = 0; p < n; p += N) {
+  __device__ __forceinline__ void add_parts(const float* ml, const float* x, int first, int step, int n) {
+    for (int p = first; p < n; p += N * step) {
       f32x2 b[N];
       f32x4 v[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int q = min(p + i, n - 1);
+        const int q = min(p + i * step, n - 1);
         b[i] = *reinterpret_cast<const f32x2*>(ml + 2 * q);
         v[i] = *reinterpret_cast<const f32x4*>(x + (int64_t)q * D);
       }
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (p + i < n) add(b[i], v[i]);
+        if (p + i * step < n) add(b[i], v[i]);
     }
   }
   __device__ __forceinline__ void store(bf16_t* out) const {
@@ -642,7 +643,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
   Rows<BY16, KT, KV8 ? D + kTail : 2 * D> rows{a, it};
   const int step = 4 * BK;
   int kv0 = it.begin + w * BK;
-  rows.ask(kv0);  // (beside the context's length: a page past it is not used)
+  if (it.begin < it.stop) rows.ask(kv0);  // (beside the context's length: a page past it is not used)
   int lim[1] = {INT_MAX}, lo, hi;
   if (it.own && it.slots == a.G) {  // one token: a limit for all
     lim[0] = lo = hi = __builtin_amdgcn_readfirstlane(slot_limit(a, it, 0));
@@ -859,19 +860,34 @@ __global__ __launch_bounds__(256, FORM == KEYS && D < 256 ? 4 : 2) void attn_sha
   }
 }
 
-template <int D>
+// Groups of D / 4 threads, four numbers a thread. TOGETHER: so many of them, a workgroup, take a (row, head)'s parts in turn and meet in
+// LDS, where there are more than 32 (32 query heads of one row behind 120000 positions, 257 parts: the call 32 us, with a group alone 61;
+// 23 rows of 64 heads with 24 parts 69 and 67, within the noise of two runs).
+template <int D, int TOGETHER>
 __global__ __launch_bounds__(256) void attn_shared_join_kernel(const SharedAttn a) {
-  constexpr int PER = D / 4;  // threads of a (row, head)
-  const int64_t i = (int64_t)blockIdx.x * (256 / PER) + threadIdx.x / PER;
-  const int d = threadIdx.x % PER * 4;
-  if (i >= (int64_t)a.T * a.nh) return;
+  constexpr int PER = D / 4, EACH = PER * TOGETHER;
+  const int64_t i = (int64_t)blockIdx.x * (256 / EACH) + threadIdx.x / EACH;
+  const int grp = threadIdx.x % EACH / PER, d = threadIdx.x % PER * 4;
   const int t = i / a.nh, h = i % a.nh;
-  if (seq_of(a, t) < 0) return;  // a row of no sequence stays as it was
+  const bool there = i < (int64_t)a.T * a.nh && seq_of(a, t) >= 0;  // (a row of no sequence stays as it was)
   Joined j;
-  const float *ml = a.pml + i * a.parts * 2, *x = a.po + i * a.parts * D + d;
-  if (a.parts <= 2) j.add_parts<D, 2>(ml, x, a.parts);
-  else j.add_parts<D, 8>(ml, x, a.parts);
-  j.store(a.out + (int64_t)t * a.out_stride + (int64_t)h * D + d);
+  if (there) {
+    const float *ml = a.pml + i * a.parts * 2, *x = a.po + i * a.parts * D + d;
+    if (TOGETHER > 1) j.add_parts<D, 4>(ml, x, grp, TOGETHER, a.parts);
+    else if (a.parts <= 2) j.add_parts<D, 2>(ml, x, 0, 1, a.parts);
+    else j.add_parts<D, 8>(ml, x, 0, 1, a.parts);
+  }
+  if constexpr (TOGETHER > 1) {
+    __shared__ __attribute__((aligned(16))) f32x4 so[256];
+    __shared__ f32x2 sml[256];
+    so[threadIdx.x] = j.o;
+    sml[threadIdx.x] = f32x2{j.top, j.l};
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int k = 1; k < TOGETHER; ++k) j.add(sml[threadIdx.x + k * PER], so[threadIdx.x + k * PER]);
+  }
+  if (there) j.store(a.out + (int64_t)t * a.out_stride + (int64_t)h * D + d);
 }
 
 struct Plan {
@@ -982,7 +998,8 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
   a.parts = parts;
   a.finish = 0;
   const int64_t pre = (int64_t)p.pre_tiles * nkv * p.pre_split, own = (int64_t)B * nkv * p.own_tiles * p.own_split;
-  const int64_t join = ((int64_t)T * nh * (D / 4) + 255) / 256;
+  const int together = parts > 32 ? 1024 / D : 1;  // (see the join kernel)
+  const int64_t join = ((int64_t)T * nh * (D / 4) * together + 255) / 256;
   if (pre + own > INT_MAX || join > INT_MAX || (int64_t)T * (nh / nkv) > INT_MAX / 2) throw std::runtime_error("attn_shared: too many rows");
   // one launch for both parts where they take the same form; else the own parts', which follow, join the prefix's results themselves
   // where each is one workgroup's
@@ -1011,7 +1028,9 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
     if (kv8) SF(D_, true, 1);                                                                     \
     else if (p.ns == 2) SF(D_, false, TWO);                                                       \
     else SF(D_, false, 1);                                                                        \
-    if (!a.finish) attn_shared_join_kernel<D_><<<(unsigned)join, 256, 0, st>>>(a);                \
+    if (a.finish) break;                                                                          \
+    if (together > 1) attn_shared_join_kernel<D_, 1024 / D_><<<(unsigned)join, 256, 0, st>>>(a);  \
+    else attn_shared_join_kernel<D_, 1><<<(unsigned)join, 256, 0, st>>>(a);                       \
   } while (0)
   switch (D) {
     case 64: SD(64); break;

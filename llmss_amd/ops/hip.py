@@ -256,8 +256,8 @@ def attn_shared(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx
     B, kv8, max_own = _ref.attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx_lens, nh, nkv, D, cu_q,
                                              max_qlen, max_own, out)
     dev = _here(q, k_cache, v_cache, prefix_table, block_tables, ctx_lens, cu_q, out)
-    qp, qs = q.data_ptr(), q.stride(0)
-    _check(qp % 16 == 0 and qs % 8 == 0 and scale > 0, "q rows must be 16-byte aligned, scale positive")
+    qp, qs, kp, vp = q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr()
+    _check((qp | kp | vp) % 16 == 0 and qs % 8 == 0 and scale > 0, "q rows and caches must be 16-byte aligned, scale positive")
     T = q.shape[0]
     y = out if out is not None else q.new_empty((T, nh * D))
     yp, ys = y.data_ptr(), y.stride(0)
@@ -268,7 +268,7 @@ def attn_shared(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx
     parts = C.attn_shared_parts(T, B, nh, nkv, D, prefix_len, max_qlen, max_own, kv8)
     ws = q.new_empty(T * nh * parts * (D + 2), dtype=torch.float32)
     nb, _, bs, _ = k_cache.shape
-    C.attn_shared(qp, qs, k_cache.data_ptr(), v_cache.data_ptr(), nb, prefix_table.data_ptr(), prefix_len, block_tables.data_ptr(),
+    C.attn_shared(qp, qs, kp, vp, nb, prefix_table.data_ptr(), prefix_len, block_tables.data_ptr(),
                   block_tables.stride(0), block_tables.shape[1], 0 if cu_q is None else cu_q.data_ptr(), ctx_lens.data_ptr(), yp, ys,
                   ws.data_ptr(), parts, T, B, nh, nkv, D, bs, max_qlen, max_own, scale, kv8, _raw_stream(dev))
     return y

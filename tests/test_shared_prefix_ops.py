@@ -218,6 +218,76 @@ def test_strided_operands(dev):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("qlens", [[1, 1, 1], [3, 1, 5]])
+def test_tables_without_pages(dev, qlens):
+    """Every context lies within the prefix (tables of no columns), or nothing is shared (a prefix of no pages)."""
+    for nh, D in ((4, 64), (2, 256), (32, 128)):
+        c = _case(dev, nh, 2, D, 90, [0, -5, -60], qlens=qlens, seed=12)
+        c["bt"] = c["bt"][:, :0]
+        _near(_run(c), c)
+        _near(_run(c, max_own=0), c)
+        c = _case(dev, nh, 2, D, 0, [9, 70, 33], qlens=qlens, seed=13)
+        assert c["ptab"].numel() == 0
+        _near(_run(c), c)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nh,nkv,D,fp8", [(2, 1, 128, False), (16, 1, 64, True), (2, 2, 256, False)])
+def test_long_contexts_of_few_rows(dev, nh, nkv, D, fp8):
+    """Many partial results a row: a prefix of a few thousand positions, and own parts as long."""
+    for owns, qlens in (([1], [1]), ([2900, 40], [1, 1]), ([2300], [20])):
+        c = _case(dev, nh, nkv, D, 3500, owns, qlens=qlens, fp8=fp8, seed=14)
+        _near(_run(c), c)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_size(dev, sign):
+    """Products of +-2^112 beside each other: all keys are the same, so every weight is, and the result is the mean of the values."""
+    for qlens in ([1, 1], [1, 30]):
+        c = _case(dev, 8, 2, 64, 50, [20, 30], qlens=qlens, seed=15)
+        c["q"][:] = sign * 2.0 ** 53
+        c["k"][:] = 2.0 ** 53
+        _near(_run(c), c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qlens", [[1, 1, 1], [4, 20, 3]])
+def test_a_cache_of_more_than_four_gigabytes(qlens):
+    """Pages at both ends of a cache whose rows lie more than 2^32 bytes apart give what the same rows give in a small one."""
+    c = _case("cuda", 8, 2, 128, 100, [4, 50, 33], qlens=qlens, seed=16)
+    want = _run(c)
+    small = c["k"].shape[0]
+    nb = 540000  # of 8 KiB each
+    k, v = (torch.empty(nb, 2, 16, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    to = torch.arange(small, device="cuda")
+    to[1::2] = nb - 1 - to[1::2]
+    k[to], v[to] = c["k"], c["v"]
+    far = lambda t: torch.where(t >= 0, to[t.clamp(min=0).long()], t.long()).int()  # noqa: E731
+    assert torch.equal(_run(dict(c, k=k, v=v, ptab=far(c["ptab"]), bt=far(c["bt"]))), want)
+
+
+@pytest.mark.gpu
+def test_rows_of_logits_past_32_bits():
+    """The last rows of logits that lie 2^32 bytes and more behind the first, and the same mask row for all."""
+    B, V = 40, 50000
+    buf = torch.empty(B, 1 << 25, dtype=torch.float32, device="cuda")
+    x = buf[:, :V]
+    x.copy_(torch.randn(B, V, generator=torch.Generator().manual_seed(3)))
+    mask = torch.full((1, (V + 31) // 32), 0x55555555, dtype=torch.int32, device="cuda")
+    rows = torch.zeros(B, dtype=torch.int32, device="cuda")
+    ids = torch.full((B, 2), V - 1, device="cuda")
+    n = torch.full((B,), 2, dtype=torch.int32, device="cuda")
+    p = torch.ones(B, device="cuda")
+    for got in (ops.adjust_logits(x, ids, n, presence=p, mask=mask, mask_rows=rows),
+                ops.adjust_logits(x, ids, n, presence=p, mask=mask, mask_rows=rows, out=torch.empty_like(buf)[:, :V])):
+        assert torch.equal(got[:, ::2], x[:, ::2]) and (got[:, 1::2] == float("-inf")).all()
+    tok = torch.full((B,), 7, device="cuda")
+    for a, b in zip(ops.token_logprobs(x, tok, 5), ops.token_logprobs(x.contiguous(), tok, 5)):
+        assert torch.equal(a, b)
+
+
 def test_attention_refusals():
     c = _case("cpu", 4, 2, 64, 33, [3, 30, 18])
 
@@ -623,3 +693,16 @@ def test_operands_of_another_place_are_refused():
     q = torch.zeros(3, c["q"].shape[1] + 4, dtype=torch.bfloat16, device="cuda")[:, 4:]
     with pytest.raises(ValueError, match="aligned"):
         _run(dict(c, q=q))
+    k = torch.zeros(c["k"].numel() + 8, dtype=torch.bfloat16, device="cuda")[4:-4].view(c["k"].shape)
+    with pytest.raises(ValueError, match="aligned"):
+        _run(dict(c, k=k))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_empty_batches(dev):
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    c = _case(dev, 4, 2, 64, 33, [3], seed=17)
+    assert _run(dict(c, q=c["q"][:0], bt=c["bt"][:0], ctx=none)).shape == (0, 256)
+    assert ops.adjust_logits(torch.zeros(0, 8, device=dev)).shape == (0, 8)
+    lp, rank, ids, top = ops.token_logprobs(torch.zeros(0, 8, device=dev), None, 3)
+    assert lp.shape == rank.shape == (0,) and ids.shape == top.shape == (0, 3)
