@@ -431,14 +431,19 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
   const int li = lane & 15, g = lane >> 4;
   int slot[NS], lim[NS];
   int lo = INT_MAX, hi = 0;
+  unsigned blind = 0;
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
     slot[n] = it.first + (w * NS + n) * 16 + li;
-    lim[n] = INT_MAX;  // (a slot behind the last: of no consequence, and no reason for a mask)
-    if (slot[n] < it.slots) {
-      lim[n] = slot_limit(a, it, slot[n]);
+    lim[n] = slot[n] < it.slots ? slot_limit(a, it, slot[n]) : 0;
+    if (lim[n] > it.begin) {
       lo = min(lo, lim[n]);
       hi = max(hi, lim[n]);
+    } else {
+      // a slot behind the last, or one that sees none of the keys (of an idle row): no reason for a mask, its sum is made zero at the
+      // end (128 rows, three of them idle, behind 16381 positions: with masks their workgroups hold the launch up, 103 us and not 84)
+      lim[n] = INT_MAX;
+      blind |= 1u << n;
     }
   }
   const int wave_lo = wave_min(lo), wave_hi = wave_max(hi);
@@ -618,7 +623,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
   for (int n = 0; n < NS; ++n) {
     meet<KV8>(lsum[n]);
     const int l = anew(), slot = it.first + (w * NS + n) * 16 + (l & 15);
-    if (slot < it.slots) leave<D>(a, it, slot, l >> 4, o[n], m[n], lsum[n][0]);
+    if (slot < it.slots) leave<D>(a, it, slot, l >> 4, o[n], m[n], blind >> n & 1 ? 0.f : lsum[n][0]);
   }
 }
 
@@ -649,7 +654,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
     lim[0] = lo = hi = __builtin_amdgcn_readfirstlane(slot_limit(a, it, 0));
   } else {
     if (real) lim[0] = slot_limit(a, it, slot);
-    lo = wave_min(lim[0]);
+    lo = wave_min(it.own || lim[0] > it.begin ? lim[0] : INT_MAX);  // (of the prefix's parts those with a sum of zero are not looked at)
     hi = wave_max(real ? lim[0] : 0);
   }
   it.stop = min(it.stop, hi);
