@@ -6,8 +6,11 @@
 // of exponentials, how many of its tokens are ahead of the given one, and its own n likeliest in order; a second launch joins a row's
 // runs. The n likeliest of a run: a number that at least n tokens reach is found from the lanes' own maxima (a binary search over the
 // upper bits of an order-preserving key, by ballots), and the few tokens that reach it are ranked by counting. Keys carry the token behind
-// the value, so no two are equal: where a run of equal logits has more than the list takes, the search goes on over all bits. A NaN counts as no candidate, and makes its row's
-// log-probabilities NaN; a row of nothing but -inf has log-probabilities of -inf.
+// the value, so no two are equal: where a run of equal logits has more than the list takes, the search goes on over all bits. A NaN
+// counts as no candidate, and makes its row's log-probabilities NaN; a row of nothing but -inf has log-probabilities of -inf. Few rows of
+// ordinary vocabularies take one launch, a workgroup a row.
+// One row of 32000 bf16 tokens 8.0 us, a chain of waits (tokens, maximum, sum, search, list); 64 of 50257 13.9, as they are one compute
+// unit's each; 256 of 131071 fp32 tokens with 20 likeliest 28.5 + 6.5, the first 4.7 TB/s.
 #include "common.h"
 
 #include <type_traits>
@@ -15,6 +18,7 @@
 namespace {
 
 constexpr int kMostTop = 64;
+constexpr float kL2e = 1.4426950408889634f;
 typedef unsigned long long u64;
 
 // ascending with the value and, among equal values, with falling token; 0 for what is not there, above it for every number (-inf too)
@@ -28,16 +32,28 @@ __device__ __forceinline__ float value_of(u64 k) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
+// A log-probability is x - base - log, from the row's maximum and its sum against it.
+__device__ __forceinline__ float base_of(float M) { return M == -INFINITY ? 0.f : M; }
+__device__ __forceinline__ float log_of(float M, float S) { return M == -INFINITY && S == 0.f ? 0.f : logf(S); }
+
 template <typename T>
 __device__ __forceinline__ float at(const T* p) {
   if constexpr (sizeof(T) == 2) return bf2f(*p);
   else return *p;
 }
 
-// NT threads, up to PACKS x 8 tokens a thread, len a run. Partial results of run c of row b: part[b][c] = (m, s, ahead, -), top[b][c][n] keys.
-template <typename T, int NT, int PACKS, bool VEC>
+struct Answers {
+  float* lp;
+  int64_t *rank, *top_ids;
+  float* top_lp;
+};
+
+// NT threads, up to PACKS x 8 tokens a thread, len a run. Partial results of run c of row b: part[b][c] = (m, s, ahead, -), top[b][c][n]
+// keys. ALONE: a row is one run, and its results are the row's.
+template <typename T, int NT, int PACKS, bool VEC, bool ALONE>
 __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ tokens, int V,
-                                                           int n, int len, int cap, float* __restrict__ part, u64* __restrict__ top) {
+                                                           int n, int len, int cap, float* __restrict__ part, u64* __restrict__ top,
+                                                           const Answers to) {
   constexpr int NW = NT / 64;
   const int b = blockIdx.y, c = blockIdx.x, runs = gridDim.x, lo = c * len, end = min(V, lo + len);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -80,13 +96,15 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
       ahead += x[k][i] > mine;
     }
   // the wave's maximum, and its sum against it (the waves' are joined at the end)
-  const float wm = warp_max(m), base = wm == -INFINITY ? 0.f : wm;
-  constexpr float kL2e = 1.4426950408889634f;
+  const float wm = warp_max(m), base = base_of(wm);
   float s = 0.f;
 #pragma unroll
-  for (int k = 0; k < PACKS; ++k)
+  for (int k = 0; k < PACKS; ++k) {  // (a pack's sum first: fewer roundings behind each other)
+    float p = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f((x[k][i] - base) * kL2e);
+    for (int i = 0; i < 8; ++i) p += __builtin_amdgcn_exp2f((x[k][i] - base) * kL2e);
+    s += p;
+  }
   s = warp_sum(s);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) ahead += __shfl_xor(ahead, o, 64);
@@ -131,6 +149,24 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
     }
   }
   __syncthreads();
+  float M = red[0], S = 0.f;
+  int A = 0;
+#pragma unroll
+  for (int i = 1; i < NW; ++i) M = fmaxf(M, red[i]);
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    // (a wave of -inf alone gives nothing; its sum may be NaN, which stays)
+    S += red[i] == -INFINITY ? reds[i] : reds[i] * __builtin_amdgcn_exp2f((red[i] - M) * kL2e);
+    A += redn[i];
+  }
+  auto give = [&](int place, u64 q) {  // (0: a row of so many NaN that there are no n others)
+    if constexpr (ALONE) {
+      to.top_ids[(int64_t)b * n + place] = q ? (int)~(unsigned)q : -1;
+      to.top_lp[(int64_t)b * n + place] = q ? value_of(q) - base_of(M) - log_of(M, S) : NAN;
+    } else {
+      top[((int64_t)b * runs + c) * n + place] = q;
+    }
+  };
   if (n > 0) {
     int have = found;
     if (have > cap) {  // (ties, or a run with few numbers: the same in every thread)
@@ -174,28 +210,22 @@ __global__ __launch_bounds__(NT) void logprobs_runs_kernel(const T* __restrict__
       __syncthreads();
       have = found;
     }
-    u64* mine_top = top + ((int64_t)b * runs + c) * n;
     for (int i = threadIdx.x; i < have; i += NT) {
       const u64 q = list[i];
-      int rank = 0;
+      int place = 0;
 #pragma unroll 8
-      for (int j = 0; j < have; ++j) rank += list[j] > q;
-      if (rank < n) mine_top[rank] = q;
+      for (int j = 0; j < have; ++j) place += list[j] > q;
+      if (place < n) give(place, q);
     }
-    for (int i = have + threadIdx.x; i < n; i += NT) mine_top[i] = 0;
+    for (int i = have + threadIdx.x; i < n; i += NT) give(i, 0);
   }
   if (threadIdx.x == 0) {
-    float M = red[0], S = 0.f;
-    int A = 0;
-#pragma unroll
-    for (int i = 1; i < NW; ++i) M = fmaxf(M, red[i]);
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      // (a wave of -inf alone gives nothing; its sum may be NaN, which stays)
-      S += red[i] == -INFINITY ? reds[i] : reds[i] * __builtin_amdgcn_exp2f((red[i] - M) * kL2e);
-      A += redn[i];
+    if constexpr (ALONE) {
+      to.lp[b] = given ? mine - base_of(M) - log_of(M, S) : 0.f;
+      to.rank[b] = given ? (int64_t)A + 1 : 0;
+    } else {
+      *reinterpret_cast<f32x4*>(part + ((int64_t)b * runs + c) * 4) = f32x4{M, S, __int_as_float(A), 0.f};
     }
-    *reinterpret_cast<f32x4*>(part + ((int64_t)b * runs + c) * 4) = f32x4{M, S, __int_as_float(A), 0.f};
   }
 }
 
@@ -219,7 +249,6 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
   float m = -INFINITY, s = 0.f;
   int ahead = 0, there = 0;
   u64 least = ~0ull, most = 0;  // of the runs' j-th keys, of their n-th ones
-  constexpr float kL2e = 1.4426950408889634f;
   for (int i = threadIdx.x; i < runs; i += 256) {
     const f32x4 p = *reinterpret_cast<const f32x4*>(part + ((int64_t)b * runs + i) * 4);
     const float t = fmaxf(m, p[0]);
@@ -274,7 +303,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
   }
   line = lj > line ? lj : line;
   if (line == 0) line = 1;
-  const float base = M == -INFINITY ? 0.f : M, ls = M == -INFINITY && S == 0.f ? 0.f : logf(S);
+  const float base = base_of(M), ls = log_of(M, S);
   if (threadIdx.x == 0) {
     lp[b] = given ? mine - base - ls : 0.f;
     rank[b] = given ? (int64_t)A + 1 : 0;
@@ -302,12 +331,18 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
   }
 }
 
-constexpr int kNT = 256;
+constexpr int kNT = 256, kAlone = 1024;
 
 // 8-token packs of a thread: four, or one while those would fill the chip less than twice and n is small against a run.
 int packs_of(int B, int V, int n) {
   return n > 20 || V > (1 << 18) || (int64_t)B * ((V + 4 * 8 * kNT - 1) / (4 * 8 * kNT)) >= 512 ? 4 : 1;
 }
+
+// Whether a row is one workgroup's, of 1024 threads with 2, 4 or 8 packs: while there is a compute unit for each (two workgroups
+// with 2 packs share one). It saves the second launch and the partial results: with a call's host steps 32000 tokens of one row 10.9 us
+// and 14.3 in two launches, 256 rows of 50257 16.9 and 21.2, 512 of 9000 13.0 and 15.0; beyond, 300 rows of 32000 17.4 and 16.3, 512 of
+// 50257 28.8 and 26.4, 1000 of 16000 23.7 and 22.4.
+bool alone(int B, int V) { return V <= kAlone * 8 * 2 ? B <= 512 : V <= kAlone * 8 * 8 && B <= 256; }
 
 // Keys that a run's list holds: several times what is found as a rule, and what the exact way may need.
 int list_of(int n, int packs) { return n == 0 ? 0 : std::max(512, n * packs * 8); }
@@ -315,41 +350,51 @@ int list_of(int n, int packs) { return n == 0 ? 0 : std::max(512, n * packs * 8)
 }  // namespace
 
 int logprobs_runs(int B, int V, int n) {
+  if (alone(B, V)) return 0;
   const int run = kNT * 8 * packs_of(B, V, n);
   return (V + run - 1) / run;
 }
-
 
 void launch_logprobs(const void* logits, int64_t ld, bool fp32, const void* tokens, int B, int V, int n, void* part, void* top, void* lp,
                      void* rank, void* top_ids, void* top_lp, hipStream_t st) {
   if (B == 0) return;
   if (B > 65535) throw std::runtime_error("token_logprobs: at most 65535 rows");
   if (n < 0 || n > kMostTop || n > V) throw std::runtime_error("token_logprobs: top_n must be between 0 and min(64, vocab)");
+  const bool vec = (uintptr_t)logits % 16 == 0 && ld * (fp32 ? 4 : 2) % 16 == 0;
+  const Answers to = {(float*)lp, (int64_t*)rank, (int64_t*)top_ids, (float*)top_lp};
+#define LK(T_, NT_, P_, V_, A_)                                                                                            \
+  logprobs_runs_kernel<T_, NT_, P_, V_, A_><<<grid, NT_, (size_t)list_of(n, P_) * 8, st>>>(                                \
+      (const T_*)logits, ld, (const int64_t*)tokens, V, n, len, list_of(n, P_), (float*)part, (u64*)top, to)
+#define LT(NT_, P_, A_)                                              \
+  do {                                                               \
+    if (fp32 && vec) LK(float, NT_, P_, true, A_);                   \
+    else if (fp32) LK(float, NT_, P_, false, A_);                    \
+    else if (vec) LK(bf16_t, NT_, P_, true, A_);                     \
+    else LK(bf16_t, NT_, P_, false, A_);                             \
+    HIP_CHECK_LAUNCH();                                              \
+  } while (0)
+  if (alone(B, V)) {
+    const dim3 grid(1, B);
+    const int len = V;
+    if (V <= kAlone * 8 * 2) LT(kAlone, 2, true);
+    else if (V <= kAlone * 8 * 4) LT(kAlone, 4, true);
+    else LT(kAlone, 8, true);
+    return;
+  }
   const int packs = packs_of(B, V, n), runs = logprobs_runs(B, V, n);
   const int len = ((V + runs - 1) / runs + 7) / 8 * 8;  // (runs of a row as long as each other: a short last one has no better line)
   const size_t join = (size_t)runs * n * 8;
   if (V >= 1 << 24 || join > 30 * 1024) throw std::runtime_error("token_logprobs: vocabulary too large");
-  const bool vec = (uintptr_t)logits % 16 == 0 && ld * (fp32 ? 4 : 2) % 16 == 0;
   const dim3 grid(runs, B);
-#define LK(T_, P_, V_)                                                                                                  \
-  logprobs_runs_kernel<T_, kNT, P_, V_><<<grid, kNT, (size_t)list_of(n, P_) * 8, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, len, list_of(n, P_), \
-                                                                                (float*)part, (u64*)top)
-#define LP(T_)                                                                                                          \
-  do {                                                                                                                  \
-    if (packs == 4) {                                                                                                   \
-      if (vec) LK(T_, 4, true);                                                                                         \
-      else LK(T_, 4, false);                                                                                            \
-    } else {                                                                                                            \
-      if (vec) LK(T_, 1, true);                                                                                         \
-      else LK(T_, 1, false);                                                                                            \
-    }                                                                                                                   \
-    HIP_CHECK_LAUNCH();                                                                                                 \
-    logprobs_join_kernel<T_><<<B, 256, 2 * join, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, runs, (const float*)part, \
-                                                   (const u64*)top, (float*)lp, (int64_t*)rank, (int64_t*)top_ids, (float*)top_lp); \
-  } while (0)
-  if (fp32) LP(float);
-  else LP(bf16_t);
-#undef LP
+  if (packs == 4) LT(kNT, 4, false);
+  else LT(kNT, 1, false);
+#define LJ(T_)                                                                                                                \
+  logprobs_join_kernel<T_><<<B, 256, 2 * join, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, runs, (const float*)part, \
+                                                     (const u64*)top, to.lp, to.rank, to.top_ids, to.top_lp)
+  if (fp32) LJ(float);
+  else LJ(bf16_t);
+#undef LJ
+#undef LT
 #undef LK
   HIP_CHECK_LAUNCH();
 }

@@ -309,8 +309,10 @@ def token_logprobs(logits, tokens, top_n=0, vocab=None):
     _check(runs * top_n * 8 <= 30 * 1024, "vocabulary too large for so many of the likeliest tokens")
     lp, tlp = logits.new_empty(B, dtype=f32), logits.new_empty((B, top_n), dtype=f32)
     rank, ids = logits.new_empty(B, dtype=i64), logits.new_empty((B, top_n), dtype=i64)
-    ws = logits.new_empty(B * runs * (2 + top_n), dtype=i64)  # (m, s, count, -) and the likeliest of each run
-    wp = ws.data_ptr()
+    wp = 0
+    if runs:  # (else one launch does it)
+        ws = logits.new_empty(B * runs * (2 + top_n), dtype=i64)  # (m, s, count, -) and the likeliest of each run
+        wp = ws.data_ptr()
     C.token_logprobs(logits.data_ptr(), logits.stride(0), logits.dtype == f32, _ptr(tokens), B, V, top_n, wp, wp + B * runs * 16,
                      lp.data_ptr(), rank.data_ptr(), ids.data_ptr(), tlp.data_ptr(), _raw_stream(dev))
     return lp, rank, ids, tlp

@@ -551,6 +551,41 @@ def test_log_probabilities_of_rows_out_of_the_ordinary(dev):
 
 
 @pytest.mark.gpu
+def test_log_probabilities_do_not_depend_on_the_batch():
+    """The same rows alone and among as many as take the other cut, over vocabularies on both sides of each cut."""
+    for V in (16384, 16385, 32768, 32769, 50257, 65536, 65537):
+        for dtype in (torch.float32, torch.bfloat16):
+            x = (torch.randn(600, V, generator=torch.Generator(device="cuda").manual_seed(V), device="cuda") * 4).to(dtype)
+            tok = torch.randint(0, V, (600,), device="cuda")
+            many = ops.token_logprobs(x, tok, 5)
+            few = ops.token_logprobs(x[:9], tok[:9], 5)
+            assert torch.equal(many[1][:9], few[1]) and torch.equal(many[2][:9], few[2])
+            want = torch.log_softmax(x[:9].cpu().double(), -1)
+            for lp, _, ids, top in (many, few):
+                _lp_near(lp[:9], want.gather(1, tok[:9, None].cpu())[:, 0])
+                _lp_near(top[:9], want.gather(1, ids[:9].cpu()))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [300, 20000, 70000])
+def test_log_probabilities_of_logits_masked_with_the_lowest_value(dev, dtype, V):
+    low = torch.finfo(dtype).min
+    x = torch.full((3, V), low).to(dtype)
+    x[0, 5], x[0, V - 1] = 2.0, 1.0
+    x[1, V // 2:V // 2 + 9] = torch.arange(9).to(dtype)
+    tok = torch.tensor([V - 1, 0, 3])
+    lp, rank, ids, top = (t.cpu() for t in ops.token_logprobs(x.to(dev), tok.to(dev), 4))
+    want = torch.log_softmax(x.double(), -1)
+    for got, w in ((lp, want[torch.arange(3), tok]), (top, want.gather(1, ids))):
+        ok = w > low / 2  # (the others are the lowest value or below it)
+        _lp_near(got[ok], w[ok])
+        assert (got[~ok] <= low * 0.99).all() and not got.isnan().any()
+    assert rank.tolist() == [2, 10, 1] and ids[0].tolist() == [5, V - 1, 0, 1] and ids[2].tolist() == [0, 1, 2, 3]
+    assert ids[1].tolist() == [V // 2 + 8 - i for i in range(4)]
+
+
+@pytest.mark.gpu
 def test_the_likeliest_of_sorted_rows():
     """Rising and falling rows put the likeliest into few threads' tokens; rows of two values are all ties."""
     V = 40001
