@@ -6,19 +6,28 @@
 //   s_j = scale q . k_j,   o = sum_j exp(s_j - M) v_j / sum_j exp(s_j - M)
 // A softmax over two sets of keys is joined from the sets' own maxima, sums and unnormalised outputs:
 //   M = max_i m_i,   o = sum_i e^(m_i - M) o_i / sum_i e^(m_i - M) l_i
-// so one launch has workgroups for the prefix (all rows of the batch against a run of its keys) and workgroups for the own
-// parts, each leaving (m, l, o) in fp32, and a second launch joins them. The prefix's share is bound by matrix instructions from
-// some 200 rows a key head on, the own parts by memory: in one launch they fill each other's gaps.
+// so the prefix (all rows of the batch against a run of its keys a workgroup) and the own parts are worked on apart, each leaving
+// (m, l, o) in fp32. The prefix's share is bound by matrix instructions and what they are fed from LDS from some 200 rows a key head on,
+// the own parts by memory.
 //
 // Both kinds take (row, query head of the key head's group) pairs as "slots", the columns of swapped products
 //   S^T[key][slot] = K Q^T,   O^T[dim][slot] += V^T P^T
 // so that a lane owns a slot's softmax (lane & 15) and P^T is made in the registers that the second product takes it from.
 // Two forms of a workgroup:
 //  rows by waves - many slots: each wave has 16 NS slots of its own, all four share tiles of keys and values in LDS (two places:
-//    the next tile is fetched while one is computed).
+//    the next tile is fetched while one is computed). A fragment from LDS feeds NS matrix instructions; two of them ask LDS for all that it
+//    gives, 128 bytes a cycle, so one group cannot pass half of the matrix rate.
 //  keys by waves - up to 16 slots (single tokens' own parts, a few rows behind a prefix): the waves walk different keys of the same
 //    slots, without a barrier, keys straight into registers, and meet at the end. One slot of 16 may be real: 64 keys of 128
-//    numbers cost a wave about 1000 cycles, memory takes 3500 to bring a compute unit's share of them.
+//    numbers cost a wave about 1000 cycles, memory takes 3500 to bring a compute unit's share of them. Few registers and 38 KB of LDS, so
+//    that four workgroups share a compute unit.
+// Together they make three kinds of call (`shared_plan`): both parts in one launch of either form and a launch that joins, or the prefix
+// by rows and then own parts by keys, which join the prefix's results themselves.
+//
+// Measured: 128 rows of 64 heads in 8 groups behind 16381 positions 84 us for the prefix (820 TFLOP/s; 256 rows
+// behind 16384 135 us, 1.0 PFLOP/s), 38 for own parts of up to 500; 64 rows of 32 heads behind 2048 positions 13.5 + 28 (own parts at
+// 4 TB/s); 16 heads of 256 with 24 questions behind 1777 positions 101 (540 TFLOP/s, near what one group a fragment allows) + 16 for the
+// join.
 //
 // Keys that a slot does not see weigh nothing whatever lies there: scores are replaced, not multiplied; rows past the last visible
 // key are never loaded (a visible one is, again); and where a tile that is masked for some slots holds values that are not finite,
@@ -628,7 +637,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
 }
 
 // ------------------------------------------------------------------------------------------------------ keys by waves
-// A wave takes every fourth run of 32 keys. Keys come straight into the first product's registers (fp8: 16 numbers a lane, so that
+// A wave takes every fourth run of 32 keys and asks for a run's keys and values together. Keys come straight into the first product's registers (fp8: 16 numbers a lane, so that
 // a pair of products shares them: dims 64 m + 16 g + 8 h of the query's row stand beside them), values through LDS places of
 // the wave's own.
 template <int D, bool KV8, bool BY16>
@@ -905,9 +914,10 @@ int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // no second round has to be waited for (one key head, 1584 slots behind 7990 positions: 525 workgroups 45 us, 500 33), each of 256 keys or
 // more. A tile of 64 keys takes 2.0 us with one group (64 slots a workgroup), 3.3 with two (128) while two workgroups share a compute
 // unit; the partial results are written and read once, at 4.5 TB/s. Two groups halve what LDS is read for, but twice the cuts fill the
-// chip with them: 128 rows of 64 heads in 8 groups behind 16381 positions 172 us with one and 141 with two, 128 rows of 32 key heads behind
-// 8000 66 and 76, one key head as above 33 and 41. fp8 rows take as long either way (their conversion is the tile's) and heads of 256
-// have no registers for two.
+// chip with them (the calls, with one and two: 128 rows of 64 heads in 8 groups behind 16381 positions 130 us and 115, 128 rows of 32 key
+// heads behind 8000 66 and 75, one key head as above 27 and 29). Heads of 64 take one: three of their workgroups share a compute unit
+// (128 rows of 32 heads in 8 groups behind 16000 37 us, with two 41). fp8 rows take as long either way (their conversion is the tile's)
+// and heads of 256 have no registers for two.
 double cut_prefix(Plan& p, int ns, int64_t slots, int nkv, int D, int P) {
   const int tile = tile_keys(D);
   p.ns = ns;
@@ -920,6 +930,20 @@ double cut_prefix(Plan& p, int ns, int64_t slots, int nkv, int D, int P) {
   return rounds * p.pre_keys / 64 * (ns == 2 ? 3.3 : 2.0) + 2.0 * slots * nkv * (D + 2) * 4 * p.pre_split / 4.5e6;
 }
 
+// Which form takes what:
+//  up to 16 slots in the whole batch: both parts by keys (one row of 32 heads in 8 groups behind 2000 positions 13.5 us, the prefix by
+//   rows 18.9; 4 rows behind 30000 27.2 and 33.6; 2 rows of fp8 behind 16000 16.8 and 29.0).
+//  own parts by keys in a launch of their own, after the prefix's, where up to 16 slots a sequence and at least 512 (sequence, key
+//   head) pairs fill the chip: each pair is then one workgroup's, and no third launch joins (64 rows of 32 key heads behind 2048 39.1 us,
+//   in one launch with the prefix by rows 43.0; 128 rows of 8 behind 16381 115 and 124; 100 fp8 rows of 8 behind 2000 30.7 and 37.2).
+//   Not where own parts are long beside the prefix, which then fill its gaps (64 rows of 8, 2000 and up to 3000 positions: 117 us apart,
+//   112 together), and not for heads of 64 (equal, or 69 together and 74) and of 256 (30 and 40: by keys two workgroups share a compute
+//   unit, not four).
+//  everything else by rows in one launch (fewer pairs: 60 rows of one key head behind 4000 18.0 us, apart 25.8; 33 rows of 48 heads on
+//   one key head behind 7990 26.1 and 31.7).
+//  no prefix: own parts of up to 16 slots by keys (64 rows of 8 key heads of up to 500 18.7 us, by rows 19.4; fp8 24.1 and 35.0).
+// Own parts are cut until there are 256 workgroups by rows beside the prefix's (20 rows of 8 key heads with 4 tokens each 24.1 us, with 512
+// 27.6, with 2048 33.3) and 512 by keys (2 rows of 8 with up to 8000 positions 15.5, with 256 19.6, with 2048 15.4).
 Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int max_own, bool kv8) {
   Plan p;
   const int64_t slots = (int64_t)T * G;
@@ -936,13 +960,13 @@ Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int m
   } else if (P > 0) {
     const double one = cut_prefix(p, 1, slots, nkv, D, P);
     Plan two = p;
-    if (!kv8 && D <= 128 && slots > 64 && cut_prefix(two, 2, slots, nkv, D, P) < one) p = two;
+    if (!kv8 && D == 128 && slots > 64 && cut_prefix(two, 2, slots, nkv, D, P) < one) p = two;
   }
   const int64_t portion = (int64_t)std::max(1, max_qlen) * G;
-  p.own_few = p.pre_few || portion <= 16 || max_qlen == 1;
+  p.own_few = p.pre_few || (portion <= 16 && (P == 0 || (D == 128 && (int64_t)B * nkv >= 512 && max_own <= P / 2)));
   p.own_tiles = up(portion, p.own_few ? 16 : 64 * p.ns);
   const int unit = p.own_few ? 128 : tile;
-  const int runs = up(512, (int64_t)B * nkv * p.own_tiles);
+  const int runs = up(p.own_few ? 512 : 256, (int64_t)B * nkv * p.own_tiles);
   const int want = std::max(1, std::min(runs, up(std::max(1, max_own), 2 * unit)));
   p.own_keys = up(up(std::max(1, max_own), want), unit) * unit;
   p.own_split = up(std::max(1, max_own), p.own_keys);
@@ -1007,8 +1031,9 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
   const int64_t join = ((int64_t)T * nh * (D / 4) * together + 255) / 256;
   if (pre + own > INT_MAX || join > INT_MAX || (int64_t)T * (nh / nkv) > INT_MAX / 2) throw std::runtime_error("attn_shared: too many rows");
   // one launch for both parts where they take the same form; else the own parts', which follow, join the prefix's results themselves
-  // where each is one workgroup's
+  // (each is one workgroup's: there are 512 pairs or more)
   const bool apart = p.own_few && !p.pre_few && pre > 0;
+  if (apart && p.own_split != 1) throw std::runtime_error("attn_shared: an own part of several workgroups cannot join the prefix's");
   const bool by16 = bs >= 16 && (bs & (bs - 1)) == 0;
 #define SA(D_, KV8_, NS_, F_, N_)                                                                 \
   do {                                                                                            \
@@ -1022,14 +1047,14 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
     if (apart) {                                     \
       SA(D_, KV8_, NS_, ROWS, pre);                  \
       a.pre_items = 0;                               \
-      a.finish = p.own_split == 1;                   \
+      a.finish = 1;                                  \
       SA(D_, KV8_, 1, KEYS, own);                    \
     } else if (p.own_few) SA(D_, KV8_, 1, KEYS, pre + own); \
     else SA(D_, KV8_, NS_, ROWS, pre + own);         \
   } while (0)
 #define SD(D_)                                                                                    \
   do {                                                                                            \
-    constexpr int TWO = D_ <= 128 ? 2 : 1; /* (no such kernel for heads of 256) */                \
+    constexpr int TWO = D_ == 128 ? 2 : 1; /* (no such kernel for other heads) */                 \
     if (kv8) SF(D_, true, 1);                                                                     \
     else if (p.ns == 2) SF(D_, false, TWO);                                                       \
     else SF(D_, false, 1);                                                                        \
