@@ -875,8 +875,8 @@ __global__ __launch_bounds__(256, FORM == KEYS && D < 256 ? 4 : 2) void attn_sha
 }
 
 // Groups of D / 4 threads, four numbers a thread. TOGETHER: so many of them, a workgroup, take a (row, head)'s parts in turn and meet in
-// LDS, where there are more than 32 (32 query heads of one row behind 120000 positions, 257 parts: the call 32 us, with a group alone 61;
-// 23 rows of 64 heads with 24 parts 69 and 67, within the noise of two runs).
+// LDS, where there are more than 12 (the calls, a group alone and together: one row of 32 heads behind 120000 positions 61 us and 32, 10
+// rows behind 4000 15.1 and 13.6, 33 rows of 48 heads behind 7990 26.3 and 25.2; with up to 12, 180 rows of 32 heads 30.2 and 32.5).
 template <int D, int TOGETHER>
 __global__ __launch_bounds__(256) void attn_shared_join_kernel(const SharedAttn a) {
   constexpr int PER = D / 4, EACH = PER * TOGETHER;
@@ -1027,7 +1027,7 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
   a.parts = parts;
   a.finish = 0;
   const int64_t pre = (int64_t)p.pre_tiles * nkv * p.pre_split, own = (int64_t)B * nkv * p.own_tiles * p.own_split;
-  const int together = parts > 32 ? 1024 / D : 1;  // (see the join kernel)
+  const int together = parts > 12 ? 1024 / D : 1;  // (see the join kernel)
   const int64_t join = ((int64_t)T * nh * (D / 4) * together + 255) / 256;
   if (pre + own > INT_MAX || join > INT_MAX || (int64_t)T * (nh / nkv) > INT_MAX / 2) throw std::runtime_error("attn_shared: too many rows");
   // one launch for both parts where they take the same form; else the own parts', which follow, join the prefix's results themselves
