@@ -49,7 +49,7 @@ void launch_adjust_logits(const void* x, int64_t ldx, bool x32, void* y, int64_t
                           int most, bool ids64, const void* lens, const void* prompts, const void* rep, const void* pres,
                           const void* freq, const void* bias_ids, const void* bias, int64_t ldb, int biases, const void* mask,
                           int64_t ldm, const void* mask_rows, int masks, hipStream_t st);
-int logprobs_runs(int B, int V, int n);
+int logprobs_runs(int B, int V);
 void launch_logprobs(const void* logits, int64_t ld, bool fp32, const void* tokens, int B, int V, int n, void* part, void* top, void* lp,
                      void* rank, void* top_ids, void* top_lp, hipStream_t st);
 bool attn_extend_two(int total, int B, int max_qlen, int nh, int nkv, int D);
@@ -368,7 +368,7 @@ PYBIND11_MODULE(_C, m) {
     launch_adjust_logits(CP(x), ldx, x32, P(y), ldy, y32, B, V, CP(ids), ldi, most, ids64, CP(lens), CP(prompts), CP(rep), CP(pres),
                          CP(freq), CP(bids), CP(bias), ldb, nb, CP(mask), ldm, CP(mrows), masks, S(st));
   });
-  m.def("logprobs_runs", &logprobs_runs);  // (rows, vocabulary, likeliest tokens asked for)
+  m.def("logprobs_runs", &logprobs_runs);  // (rows, vocabulary); 0: one launch does it
   m.def("token_logprobs", [](uintptr_t lg, int64_t ld, bool fp32, uintptr_t tok, int B, int V, int n, uintptr_t part, uintptr_t top,
                              uintptr_t lp, uintptr_t rank, uintptr_t tid, uintptr_t tlp, uintptr_t st) {
     launch_logprobs(CP(lg), ld, fp32, CP(tok), B, V, n, P(part), P(top), P(lp), P(rank), P(tid), P(tlp), S(st));

@@ -9,8 +9,10 @@
 // in a word) up to 32767 known tokens and 32 beyond, with a bit for "seen"; the run's biases as a list in their order. The logits are
 // asked for first and come meanwhile; then the run goes through with 16-byte accesses, and only tokens whose counter is not zero cost more
 // than a copy. Biased tokens are written once more at the end, by a thread each (found in the stream, by a table of them in LDS, 300
-// biases a row cost 256 x 131071 fp32 logits 27 us beside 48). Integer counts, and biases summed in the order of the list: the result does
-// not depend on the order in which threads run.
+// biases a row cost 256 x 131071 fp32 logits 27 us beside 48, written once more 6). Integer counts, and biases summed in the order of the
+// list: the result does not depend on the order in which threads run.
+// 256 rows of 131071 fp32 logits 48 us as they are (5.6 TB/s), with up to 8000 known tokens, 300 biases and a mask 67; 64 of 50257 in bf16 with
+// up to 1000 known tokens 9.6, one of 32000 3.9, a chain of waits.
 #include "common.h"
 
 #include <type_traits>
@@ -266,6 +268,8 @@ __global__ __launch_bounds__(kThreads) void adjust_logits_kernel(const LogitRule
 template <typename TI, typename TO>
 void launch_rules(const LogitRules& a, int B, bool w16, hipStream_t st) {
   const bool vec = ((uintptr_t)a.x | (uintptr_t)a.y) % 16 == 0 && a.ldx * sizeof(TI) % 16 == 0 && a.ldy * sizeof(TO) % 16 == 0;
+  // Runs as long as 1024 workgroups or more are left: a run's workgroup walks all that is known of the row (64 rows of 50257 with 500
+  // known tokens 12.0 us, with 256 workgroups 12.6, with 4096 14.9; 256 of 131071 52.6, with 256 52.8, with 4096 51.0).
   int CH = 1024;
   while (CH < (w16 ? kMostRun : kMostRun / 2) && (int64_t)B * ((a.V + CH - 1) / CH) > 1024) CH *= 2;
   const dim3 grid((a.V + CH - 1) / CH, B);

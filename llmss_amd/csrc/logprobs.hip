@@ -331,12 +331,10 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const T* __restrict_
   }
 }
 
-constexpr int kNT = 256, kAlone = 1024;
-
-// 8-token packs of a thread: four, or one while those would fill the chip less than twice and n is small against a run.
-int packs_of(int B, int V, int n) {
-  return n > 20 || V > (1 << 18) || (int64_t)B * ((V + 4 * 8 * kNT - 1) / (4 * 8 * kNT)) >= 512 ? 4 : 1;
-}
+// Threads and 8-token packs of a thread where a row is several runs. (Runs of one pack, for few rows: 2 rows of 131071 with the
+// likeliest token 14.7 us and 15.1, 20 rows with 5 14.1 and 14.9, but 2 rows with 20 22.4 and 14.7: one form does for all.)
+constexpr int kNT = 256, kPacks = 4;
+constexpr int kAlone = 1024;  // threads where a row is one run
 
 // Whether a row is one workgroup's, of 1024 threads with 2, 4 or 8 packs: while there is a compute unit for each (two workgroups
 // with 2 packs share one). It saves the second launch and the partial results: with a call's host steps 32000 tokens of one row 10.9 us
@@ -349,9 +347,9 @@ int list_of(int n, int packs) { return n == 0 ? 0 : std::max(512, n * packs * 8)
 
 }  // namespace
 
-int logprobs_runs(int B, int V, int n) {
+int logprobs_runs(int B, int V) {
   if (alone(B, V)) return 0;
-  const int run = kNT * 8 * packs_of(B, V, n);
+  constexpr int run = kNT * 8 * kPacks;
   return (V + run - 1) / run;
 }
 
@@ -381,13 +379,12 @@ void launch_logprobs(const void* logits, int64_t ld, bool fp32, const void* toke
     else LT(kAlone, 8, true);
     return;
   }
-  const int packs = packs_of(B, V, n), runs = logprobs_runs(B, V, n);
+  const int runs = logprobs_runs(B, V);
   const int len = ((V + runs - 1) / runs + 7) / 8 * 8;  // (runs of a row as long as each other: a short last one has no better line)
   const size_t join = (size_t)runs * n * 8;
   if (V >= 1 << 24 || join > 30 * 1024) throw std::runtime_error("token_logprobs: vocabulary too large");
   const dim3 grid(runs, B);
-  if (packs == 4) LT(kNT, 4, false);
-  else LT(kNT, 1, false);
+  LT(kNT, kPacks, false);
 #define LJ(T_)                                                                                                                \
   logprobs_join_kernel<T_><<<B, 256, 2 * join, st>>>((const T_*)logits, ld, (const int64_t*)tokens, V, n, runs, (const float*)part, \
                                                      (const u64*)top, to.lp, to.rank, to.top_ids, to.top_lp)

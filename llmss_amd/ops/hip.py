@@ -305,7 +305,7 @@ def token_logprobs(logits, tokens, top_n=0, vocab=None):
     _check(B <= 65535 and V < 1 << 24, "at most 65535 rows and 2 ** 24 - 1 tokens")
     C = lib()
     f32, i64 = torch.float32, torch.int64
-    runs = C.logprobs_runs(B, V, top_n)
+    runs = C.logprobs_runs(B, V)
     _check(runs * top_n * 8 <= 30 * 1024, "vocabulary too large for so many of the likeliest tokens")
     lp, tlp = logits.new_empty(B, dtype=f32), logits.new_empty((B, top_n), dtype=f32)
     rank, ids = logits.new_empty(B, dtype=i64), logits.new_empty((B, top_n), dtype=i64)
