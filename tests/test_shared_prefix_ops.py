@@ -207,6 +207,21 @@ def test_empty_portions_and_hints_that_are_too_small(dev):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("G", [1, 20])
+def test_rows_in_front_of_the_first_sequence_stay_and_contexts_end_with_the_table(dev, G):
+    c = _case(dev, 2 * G, 2, 64, 40, [3, 30, 48], qlens=[3, 2, 1], seed=18)
+    want = _run(c)
+    q = torch.cat([torch.full_like(c["q"][:2], float("nan")), c["q"]])
+    out = torch.full((8, 2 * G * 64), 7.0, dtype=torch.bfloat16, device=dev)
+    ctx = c["ctx"].clone()
+    ctx[2] += 1000  # (its table holds 48 positions; the others' rows must not move)
+    _run(dict(c, q=q, ctx=ctx), cu_q=c["cu"] + 2, out=out)
+    assert (out[:2] == 7).all()
+    _near(out[2:7], dict(c, q=q[2:7], qlens=[3, 2]))
+    assert torch.equal(out[7], want[5])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_strided_operands(dev):
     c = _case(dev, 4, 2, 64, 33, [3, 30, 18], seed=9)
     want = _run(c)
@@ -438,6 +453,26 @@ def test_rules_pass_on_what_is_not_finite(dev):
     for row, last in zip(got, (1.5, 3.0)):
         assert row[0].isnan() and row[1] == float("inf") and row[2] == float("-inf") and row[3] == 0 and row[4] == last
         assert (row[5:] == float("-inf")).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rules_pass_over_what_is_out_of_range(dev):
+    lo64, hi64, lo32, hi32 = -2 ** 63, 2 ** 63 - 1, -2 ** 31, 2 ** 31 - 1
+    V = 3000
+    x = torch.randn(4, V, generator=torch.Generator().manual_seed(4)).to(dev)
+    ids = torch.tensor([[lo64, hi64, V, -1, 2500, lo32, hi32, 7]] * 4).to(dev)
+    lens = torch.tensor([8, hi32, -5, 5], dtype=torch.int32, device=dev)
+    prompts = torch.tensor([lo32, 5, 3, hi32], dtype=torch.int32, device=dev)
+    bids = torch.tensor([[lo32, hi32, V, 2999]] * 4, dtype=torch.int32, device=dev)
+    mask = torch.zeros(1, 94, dtype=torch.int32, device=dev)
+    got = ops.adjust_logits(x, ids, lens, prompts, presence=torch.full((4,), 0.5, device=dev), bias_ids=bids,
+                            bias=torch.ones(4, 4, device=dev), mask=mask,
+                            mask_rows=torch.tensor([lo32, hi32, 1, -1], dtype=torch.int32, device=dev))
+    want = x.clone()
+    want[:, 2999] += 1
+    want[0, [2500, 7]] -= 0.5  # all behind the prompt; of the second row 7 alone, of the others none
+    want[1, 7] -= 0.5
+    assert torch.equal(got, want)
 
 
 @pytest.mark.gpu
