@@ -66,12 +66,12 @@ def _run(c, **kw):
     return ops.attn_shared(c["q"], c["k"], c["v"], c["ptab"], c["prefix"], c["bt"], c["ctx"], c["nh"], c["nkv"], c["D"], c["scale"], **kw)
 
 
-def _plain(c):
+def _plain(c, dev="cpu"):
     """In 64 bits, a row at a time: (result, A = sum p |v|)."""
-    c = {n: x.cpu() if torch.is_tensor(x) else x for n, x in c.items()}
+    c = {n: x.to(dev if n in "qkv" else "cpu") if torch.is_tensor(x) else x for n, x in c.items()}
     nh, nkv, D, bs, P = c["nh"], c["nkv"], c["D"], c["bs"], c["prefix"]
     T = c["q"].shape[0]
-    out, A = torch.zeros(T, nh, D, dtype=F64), torch.zeros(T, nh, D, dtype=F64)
+    out, A = torch.zeros(T, nh, D, dtype=F64, device=dev), torch.zeros(T, nh, D, dtype=F64, device=dev)
     t = 0
     for b, n in enumerate(c["qlens"]):
         for i in range(n):
@@ -88,11 +88,11 @@ def _plain(c):
                 out[t] = (w[..., None] * vv).sum(0)
                 A[t] = (w[..., None] * vv.abs()).sum(0)
             t += 1
-    return out.view(T, -1), A.view(T, -1)
+    return out.view(T, -1).cpu(), A.view(T, -1).cpu()
 
 
-def _near(got, c, rows=None):
-    want, A = _plain(c)
+def _near(got, c, rows=None, dev="cpu"):
+    want, A = _plain(c, dev)
     got = got.cpu().to(F64)
     if rows is not None:
         got, want, A = got[rows], want[rows], A[rows]
@@ -231,6 +231,38 @@ def test_strided_operands(dev):
     tables[:, 4:4 + c["bt"].shape[1]] = c["bt"]
     got = _run(dict(c, q=wide[:, 64:], bt=tables[:, 4:4 + c["bt"].shape[1]]))
     assert torch.equal(got, want)
+
+
+def _many(B, several):
+    """Own parts and portions of B sequences: idle ones, contexts that end in the prefix, one token to some pages."""
+    owns = [(1, 20, 37, None, -30, 90, 64, 16, 33, 5)[i % 10] for i in range(B)]
+    qlens = [1] * B if not several else [min(1 + i % several, max(1, o or 0)) for i, o in enumerate(owns)]
+    return owns, qlens
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("nh,several,bs", [(8, 0, 16), (16, 0, 5), (24, 3, 16), (16, 7, 48)])
+def test_many_sequences_of_several_key_heads(fp8, nh, several, bs):
+    """640 (sequence, key head) pairs: own parts in a launch that joins the prefix's results."""
+    owns, qlens = _many(80, several)
+    c = _case("cuda", nh, 8, 128, 200, owns, qlens=qlens, bs=bs, fp8=fp8, seed=19)
+    _near(_run(c), c, dev="cuda")
+    if several:
+        _near(_run(c, max_qlen=1), c, dev="cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nh,nkv,D,several,parts", [(256, 32, 128, 0, 3), (256, 32, 128, 4, 3), (256, 32, 64, 0, 2)])
+def test_many_rows_of_many_heads(nh, nkv, D, several, parts):
+    """Enough rows that each wave takes two groups of them (heads of 128; single tokens: the prefix in two runs, own parts in one)."""
+    from llmss_amd.ops import hip
+
+    owns, qlens = _many(100, several)
+    c = _case("cuda", nh, nkv, D, 2400, owns, qlens=qlens, seed=20)
+    q = c["q"].shape[0]
+    assert several or hip.lib().attn_shared_parts(q, 100, nh, nkv, D, 2400, 1, c["bt"].shape[1] * 16, False) == parts
+    _near(_run(c), c, dev="cuda")
 
 
 @pytest.mark.parametrize("dev", DEVICES)
