@@ -274,8 +274,8 @@ def attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_table
         max_own = room
     _need(isinstance(max_own, int) and 0 <= max_own <= room, "max_own must be between 0 and what a row of block_tables holds")
     if out is not None:
-        _need(out.dtype == bf16 and out.dim() == 2 and out.shape[0] >= T and out.shape[1] >= nh * D and out.stride(1) == 1,
-              "out bf16 [>= T, >= nh * D]")
+        _need(out.dtype == bf16 and out.dim() == 2 and out.shape[0] >= T and out.shape[1] >= nh * D and out.stride(1) == 1
+              and (T <= 1 or out.stride(0) >= nh * D), "out bf16 [>= T, >= nh * D], rows apart")
     return B, kv8, max_own
 
 
@@ -358,7 +358,8 @@ def adjust_logits_check(logits, ids, lens, prompt_lens, repetition, presence, fr
                   "mask_rows int32 [B]")
     if out is not None:
         _need(out.dim() == 2 and out.shape[0] >= B and out.shape[1] >= V and (out.shape[1] <= 1 or out.stride(1) == 1)
-              and out.dtype in (logits.dtype, torch.float32), "out [B, >= vocab] in the type of logits or fp32, dense rows")
+              and (B <= 1 or out.stride(0) >= V) and out.dtype in (logits.dtype, torch.float32),
+              "out [B, >= vocab] in the type of logits or fp32, dense rows apart")
     return B, V
 
 
