@@ -209,13 +209,25 @@ __device__ __forceinline__ s16x8 v_fragment(const char* img, int r32, int dt, in
   return s16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
 }
 
+// The scale of row `r` of an fp8 tile of N rows, and its reciprocal behind the N scales. Scales below 2^-100 count as that (their rows hold
+// nothing above 4e-28); a reciprocal of what is not finite is 0, as such a scale may belong to a row that is not seen.
+template <int N>
+__device__ __forceinline__ void keep_scale(float* at, int r, float scale) {
+  if (fabsf(scale) < 0x1p-100f) scale = 0x1p-100f;
+  at[r] = scale;
+  const float inv = fabsf(scale) < INFINITY ? __builtin_amdgcn_rcpf(scale) : 0.f;
+  bf16_t* const two = reinterpret_cast<bf16_t*>(at + N);
+  const bf16_t hi = f2bf(inv);
+  two[r] = hi;
+  two[N + r] = f2bf(inv - bf2f(hi));
+}
+
 // Scores of 16 KT keys and NS groups of slots become weights: the running maximum of a slot moves only where its own has grown by
 // more than 8 (weights stay below 2^8), so most tiles exchange nothing between lanes and rescale nothing. Weights are rounded to
 // bf16 for the second product (half a step of 2^-8, as any bf16 operand); their sum is taken of the rounded ones, by a product with
-// ones, so that they add up to 1 as they are used. fp8 rows: a weight times its row's scale is what is rounded, so the sum is of the
-// weights themselves, by lane (the lanes of a slot meet at the end): 0.0023 from 64 bits where bf16 rows are at 0.0018. (The rounded ones
-// over their scales in the sum would make it 0.0018 as well, for 69 us instead of 64 at 23 rows behind 30011 positions, and registers that
-// the second form does not have, 41 us instead of 31.) lim: keys [.., lim) are seen, counted from the tile's first.
+// ones, so that they add up to 1 as they are used. fp8 rows: a weight times its row's scale (vscale) is what is rounded, so in place of the
+// ones stand the scales' reciprocals, in two bf16 numbers that hold 16 bits of them (behind the scales, see `keep_scale`). Against 64 bits
+// 0.0019; with a sum of the weights as they were, 0.0024 and for peaked rows 0.0027. lim: keys [.., lim) are seen, counted from the tile's first.
 template <int D, int KT, int NS, bool MASK, bool KV8>
 __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS], float scale_log2, int g, float (&m)[NS],
                                        f32x4 (&lsum)[NS], f32x4 (&o)[NS][D / 16], s16x8 (&pf)[NS][KT / 2], const float* vscale) {
@@ -262,7 +274,6 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS],
         const float p = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i], scale_log2, nm));
         short w;
         if constexpr (KV8) {
-          lsum[n][i] += p;
           w = (short)f2bf(p * v[i]);
           if (MASK && p == 0.f) w = 0;  // (a key that is not seen: its scale may be anything)
         } else {
@@ -271,9 +282,18 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS],
         pf[n][kt >> 1][(kt & 1) * 4 + i] = w;
       }
     }
-    if constexpr (!KV8) {
 #pragma unroll
-      for (int k = 0; k < KT / 2; ++k) lsum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[n][k], lsum[n], 0, 0, 0);
+    for (int k = 0; k < KT / 2; ++k) {
+      if constexpr (KV8) {
+        const short* const two = reinterpret_cast<const short*>(vscale + 16 * KT) + 32 * k + 4 * g;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const s16x4 x = *reinterpret_cast<const s16x4*>(two + h * 16 * KT), y = *reinterpret_cast<const s16x4*>(two + h * 16 * KT + 16);
+          lsum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, pf[n][k], lsum[n], 0, 0, 0);
+        }
+      } else {
+        lsum[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pf[n][k], lsum[n], 0, 0, 0);
+      }
     }
   }
 }
@@ -400,15 +420,6 @@ __device__ __forceinline__ void add_parts(const float* ml, const float* x, int f
     for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[dt][e] = o[dt][e] * f + w[dt][e] * h;
-  }
-}
-
-// The sum of a slot's weights, in all four places, where it is kept by lane.
-template <bool KV8>
-__device__ __forceinline__ void meet(f32x4& lsum) {
-  if constexpr (KV8) {
-    const float l = xor32_sum(xor16_sum((lsum[0] + lsum[1]) + (lsum[2] + lsum[3])));
-    lsum = f32x4{l, l, l, l};
   }
 }
 
@@ -552,7 +563,8 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
           *reinterpret_cast<s16x8*>(sk + TILE + at) = fp8_to_bf16(v8[i][2 * h], v8[i][2 * h + 1]);
         }
       }
-      if (threadIdx.x < 2 * BKV) scales[(j & 1) * 2 * BKV + threadIdx.x] = sc;
+      if (threadIdx.x < BKV) scales[(j & 1) * 3 * BKV + threadIdx.x] = sc;
+      else if (threadIdx.x < 2 * BKV) keep_scale<BKV>(scales + (j & 1) * 3 * BKV + BKV, threadIdx.x - BKV, sc);
     };
     auto tile = [&](int j, auto mask_c) {
       constexpr bool MASK = decltype(mask_c)::value;
@@ -580,7 +592,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
       __builtin_amdgcn_sched_barrier(0);
       const float* vs = nullptr;
       if constexpr (KV8) {
-        const float* ks_ = scales + (j & 1) * 2 * BKV;
+        const float* ks_ = scales + (j & 1) * 3 * BKV;
         vs = ks_ + BKV;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
@@ -632,7 +644,6 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
   }
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
-    meet<KV8>(lsum[n]);
     const int l = anew(), slot = it.first + (w * NS + n) * 16 + (l & 15);
     if (slot < it.slots) leave<D>(a, it, slot, l >> 4, o[n], m[n], blind >> n & 1 ? 0.f : lsum[n][0]);
   }
@@ -686,7 +697,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
     }
     char* const img = smem + w * TILE;
     const unsigned img_at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LDS_AS char*)img);
-    float* const fac = scales + w * 2 * BK;  // (fp8) scales of the keys, of the values
+    float* const fac = scales + w * 3 * BK;  // (fp8) scales of the keys, of the values, what is kept behind those
     s16x8 kf[KT][KV8 ? 1 : D / 32];
     u32x4 k8[KT][KV8 ? D / 64 : 1];
     constexpr int RPI = 64 / CH, INS = BK / RPI, PIECES = BK * (D / 16) / 64;
@@ -749,7 +760,8 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
           for (int h = 0; h < 2; ++h)
             *reinterpret_cast<s16x8*>(img + r * D * 2 + (swz<D>(c0 + h, r) << 4)) = fp8_to_bf16(v8[i][2 * h], v8[i][2 * h + 1]);
         }
-        fac[lane] = sc;
+        if (lane < BK) fac[lane] = sc;
+        else keep_scale<BK>(fac + BK, lane - BK, sc);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
       f32x4 s[1][KT];
@@ -782,7 +794,6 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the place is read)
     }
   }
-  meet<KV8>(lsum[0]);
   const bool finish = it.own && a.finish;
   if (finish) {  // the own part is one workgroup's: the prefix's parts, left by the launch before, join it here, every fourth a wave
     const int l = anew(), slot = it.first + (l & 15), g = l >> 4;
@@ -833,7 +844,7 @@ __global__ __launch_bounds__(256, FORM == KEYS && D < 256 ? 4 : 2) void attn_sha
   constexpr int PLACES = FORM == ROWS ? 2 * 2 * tile_keys(D) * D * 2 : 4 * 32 * D * 2;  // tiles; each wave's values
   constexpr int MEET = FORM == ROWS ? 0 : 4 * 16 * (D + 4) * 4;                         // the second form's outputs
   __shared__ __attribute__((aligned(16))) char smem[PLACES > MEET ? PLACES : MEET];
-  __shared__ __attribute__((aligned(16))) float scales[FORM == ROWS ? (KV8 ? 2 * 2 * tile_keys(D) : 4) : 4 * 2 * 32];
+  __shared__ __attribute__((aligned(16))) float scales[FORM == ROWS ? (KV8 ? 2 * 3 * tile_keys(D) : 4) : 4 * 3 * 32];
   __shared__ __attribute__((aligned(16))) bf16_t apart[4 * 16 * (FORM == KEYS ? 32 : tile_keys(D))];
   __shared__ int red[4];
   constexpr int per = FORM == KEYS ? 16 : 64 * NS;

@@ -299,6 +299,19 @@ def test_scores_of_any_size(dev, sign):
         _near(_run(c), c)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("qlens", [[1, 1, 1], [3, 20, 5]])
+def test_fp8_rows_of_zeros_and_of_any_scale(dev, qlens):
+    """A row whose scale is 0 has its weight all the same; scales from 1e-20 to 1e20 beside each other."""
+    c = _case(dev, 8, 2, 128, 70, [5, 30, 40], qlens=qlens, fp8=True, seed=21, poison=False)
+    for j, scale in ((3, 0.0), (40, 0.0), (50, 1e-20), (60, 1e20), (66, 1e-37)):
+        row = c["v"][c["ptab"][j // 16], :, j % 16]
+        if scale == 0:
+            row[:, :128] = 0
+        row[:, 128:132] = torch.tensor([scale]).view(torch.uint8).to(dev)
+    _near(_run(c), c)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("qlens", [[1, 1, 1], [4, 20, 3]])
 def test_a_cache_of_more_than_four_gigabytes(qlens):
@@ -362,6 +375,7 @@ def test_attention_refusals():
     no("cu_q", cu_q=c["cu"].long())
     no("max_own", max_own=1000)
     no("out", out=torch.zeros(2, 256, dtype=torch.bfloat16))
+    no("out", out=torch.zeros(1, 256, dtype=torch.bfloat16).expand(3, 256))
     no("scale", scale=0.0)
 
 
@@ -561,6 +575,7 @@ def test_rules_refusals():
     no("mask", x, mask=torch.zeros(1, 2, dtype=torch.int32))
     no("out", x, out=torch.zeros(2, 63))
     no("out", x, out=x.bfloat16())
+    no("out", x, out=x[:1].expand(2, 64))
 
 
 # -------------------------------------------------------------------------------------------------------------- logprobs
