@@ -222,14 +222,20 @@ __device__ __forceinline__ void keep_scale(float* at, int r, float scale) {
   two[N + r] = f2bf(inv - bf2f(hi));
 }
 
+// A maximum whose steps are 2 or more (not the one before any key was seen).
+__device__ __forceinline__ bool far_off(float m) { return fabsf(m) >= 0x1p24f && m != kFloor; }
+
 // Scores of 16 KT keys and NS groups of slots become weights: the running maximum of a slot moves only where its own has grown by
 // more than 8 (weights stay below 2^8), so most tiles exchange nothing between lanes and rescale nothing. Weights are rounded to
 // bf16 for the second product (half a step of 2^-8, as any bf16 operand); their sum is taken of the rounded ones, by a product with
 // ones, so that they add up to 1 as they are used. fp8 rows: a weight times its row's scale (vscale) is what is rounded, so in place of the
 // ones stand the scales' reciprocals, in two bf16 numbers that hold 16 bits of them (behind the scales, see `keep_scale`). Against 64 bits
 // 0.0019; with a sum of the weights as they were, 0.0024 and for peaked rows 0.0027. lim: keys [.., lim) are seen, counted from the tile's first.
+// An exponent is s scale - m in one rounding, while m is the rounded product: off by up to half a step of m, the same for every key of the
+// slot, so that it cancels, but from 2^31 on it would take the weights out of range. From 2^24 on (`far`, the same for all lanes of the wave, looked
+// at where a maximum moves) the product is rounded first, and the largest key's exponent is 0.
 template <int D, int KT, int NS, bool MASK, bool KV8>
-__device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS], float scale_log2, int g, float (&m)[NS],
+__device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS], float scale_log2, int g, float (&m)[NS], int& far,
                                        f32x4 (&lsum)[NS], f32x4 (&o)[NS][D / 16], s16x8 (&pf)[NS][KT / 2], const float* vscale) {
   float mx[NS];
   bool grew = false;
@@ -246,13 +252,15 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS],
     mx[n] *= scale_log2;
     grew |= mx[n] > m[n] + 8.f;
   }
-  if (__ballot(grew)) {
+  if (__ballot(grew || far)) {
+    bool any = false;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       const float top = xor32_max(xor16_max(mx[n]));
       const bool up = top > m[n] + 8.f;
       const float alpha = up ? __builtin_amdgcn_exp2f(m[n] - top) : 1.f;
       if (up) m[n] = top;
+      any |= far_off(m[n]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) lsum[n][i] *= alpha;
 #pragma unroll
@@ -260,18 +268,32 @@ __device__ __forceinline__ void soften(f32x4 (&s)[NS][KT], const int (&lim)[NS],
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][i][e] *= alpha;
     }
+    far = __ballot(any) != 0;
+    if (far) {  // (slots near 0 beside them keep their one rounding)
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float p = s[n][kt][i] * scale_log2;
+            asm("" : "+v"(p));  // (or the difference is taken in one rounding with it)
+            s[n][kt][i] = far_off(m[n]) ? p - m[n] : fmaf(s[n][kt][i], scale_log2, -m[n]);
+          }
+    }
   }
+  const float by = far ? 1.f : scale_log2;
   const s16x8 ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80};
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
-    const float nm = -m[n];
+    const float nm = far ? 0.f : -m[n];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
       f32x4 v;
       if constexpr (KV8) v = *reinterpret_cast<const f32x4*>(vscale + kt * 16 + 4 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i], scale_log2, nm));
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i], by, nm));
         short w;
         if constexpr (KV8) {
           w = (short)f2bf(p * v[i]);
@@ -476,6 +498,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
 
   f32x4 o[NS][D / 16], lsum[NS];
   float m[NS];
+  int far = 0;
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
     m[n] = kFloor;
@@ -607,7 +630,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
 #pragma unroll
       for (int n = 0; n < NS; ++n) left[n] = MASK ? min(lim[n], it.stop) - kv0 : BKV;
       s16x8 pf[NS][KT / 2];
-      soften<D, KT, NS, MASK, KV8>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
+      soften<D, KT, NS, MASK, KV8>(s, left, a.scale_log2, g, m, far, lsum, o, pf, vs);
       add_values<D, KT, NS, false>(MASK, sk + TILE, apart + w * 16 * BKV, left, g, li, pf, o);
     };
     // tiles that every slot of the wave sees whole come first, in a loop without masks
@@ -683,6 +706,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
 
   f32x4 o[1][D / 16], lsum[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
   float m[1] = {kFloor};
+  int far = 0;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) o[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   __syncthreads();  // (a workgroup may have had an item before: the places below are free)
@@ -788,7 +812,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       const float* vs = KV8 ? fac + BK : nullptr;
       s16x8 pf[1][1];
       const int left[1] = {min(lim[0], it.stop) - kv0};
-      soften<D, KT, 1, true, KV8>(s, left, a.scale_log2, g, m, lsum, o, pf, vs);
+      soften<D, KT, 1, true, KV8>(s, left, a.scale_log2, g, m, far, lsum, o, pf, vs);
       const int l = anew();
       add_values<D, KT, 1, true>(kv0 + BK > min(lo, it.stop), img, apart + w * 16 * BK, left, l >> 4, l & 15, pf, o);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the place is read)

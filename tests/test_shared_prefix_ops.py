@@ -300,6 +300,44 @@ def test_scores_of_any_size(dev, sign):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("size", [20, 24, 32, 40, 60, 100])
+@pytest.mark.parametrize("nh,nkv,D,owns,qlens", [
+    (8, 2, 128, [40, 30], [1, 1]),            # the whole batch by keys, two parts
+    (8, 2, 128, [40, 30, 9], [9, 30, 1]),     # by rows
+    (48, 1, 128, [40, 30, 70], [1, 1, 1]),
+    (4, 4, 64, [40, 30, 70], [9, 30, 1]),
+    (2, 2, 256, [40, 30, 70], [9, 30, 1]),
+    (8, 8, 128, [1 + i % 40 for i in range(70)], [1] * 70),  # the prefix by rows, own parts by keys
+])
+def test_large_scores_that_differ(dev, fp8, size, nh, nkv, D, owns, qlens):
+    """Scores of some 2^(size + 3) that are no powers of two and lie far apart: the largest takes all, whatever the rounding of its
+    exponent is by itself. With these seeds the largest is ahead by 2^-15.3 of sum |q k| and more (heads of 256 2^-13.3), and two sums
+    of D products in 32 bits are off by 2 D 2^-24 of it at most (2^-16, 2^-15): what is left, at a sum of 2^27 from the smallest size on,
+    is an exponent of 100."""
+    c = _case(dev, nh, nkv, D, 600, owns, qlens=qlens, fp8=fp8, seed=23 if fp8 else 22)
+    c["q"] = (c["q"].float() * 2.0 ** size).bfloat16()
+    want, A = _plain(c)  # (one key's value, as it is)
+    assert ((want.abs() - A).abs() <= 2.0 ** -30 * A).all()
+    _near(_run(c), c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [24, 40])
+def test_large_scores_of_many_rows_of_many_heads(size):
+    """The same where a wave takes two groups of rows: a key head's queries are one direction times powers of two, so that its keys are in one
+    order. The largest is ahead by 2^-9.9 of sum |q k| with this seed (the sums are off by 2^-16 of it)."""
+    owns, qlens = _many(100, 0)
+    c = _case("cuda", 256, 32, 128, 2400, owns, qlens=qlens, seed=24)
+    g = torch.Generator().manual_seed(24)
+    lean = torch.randn(1, 32, 1, 128, generator=g) * 1.5
+    c["q"] = (lean * 2.0 ** (size + torch.randint(0, 4, (100, 32, 8, 1), generator=g))).reshape(100, -1).bfloat16().cuda()
+    want, A = _plain(c, "cuda")
+    assert ((want.abs() - A).abs() <= 2.0 ** -30 * A).all()
+    _near(_run(c), c, dev="cuda")
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("qlens", [[1, 1, 1], [3, 20, 5]])
 def test_fp8_rows_of_zeros_and_of_any_scale(dev, qlens):
     """A row whose scale is 0 has its weight all the same; scales from 1e-20 to 1e20 beside each other."""
