@@ -377,11 +377,17 @@ __device__ __forceinline__ void add_values(bool masked, const char* img, bf16_t*
   if constexpr (!FEW) read_ahead<KT / 2 * (D / 16) * 2, 8, 2, NS>();
 }
 
+// A sum of no weights is left as -0, one of weights of zero (keys of -inf) as +0, so that a row that sees nothing gets zeros and one that
+// sees keys of -inf alone, and has no softmax, 0 / 0.
+constexpr unsigned kNone = 0x80000000u;
+
 // A softmax over several sets of keys from the sets' (m, l) and four of their outputs.
 struct Joined {
   float top = kFloor, l = 0.f;
+  unsigned none = kNone;  // (as long as every set's sum is -0)
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   __device__ __forceinline__ void add(f32x2 ml, f32x4 x) {
+    none &= __float_as_uint(ml[1]);
     if (ml[1] == 0.f) return;  // (a set without a visible key; its outputs may be anything)
     const float t = fmaxf(top, ml[0]), f = __builtin_amdgcn_exp2f(top - t), h = __builtin_amdgcn_exp2f(ml[0] - t);
     top = t;
@@ -406,8 +412,9 @@ struct Joined {
         if (p + i * step < n) add(b[i], v[i]);
     }
   }
+  __device__ __forceinline__ float sum() const { return l == 0.f ? __uint_as_float(none) : l; }
   __device__ __forceinline__ void store(bf16_t* out) const {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = __float_as_uint(sum()) == kNone ? 0.f : 1.f / l;
     u16x4 r;
 #pragma unroll
     for (int e = 0; e < 4; ++e) r[e] = f2bf(o[e] * inv);
@@ -426,6 +433,7 @@ __device__ __forceinline__ void add_parts(const float* ml, const float* x, int f
     for (int dt = 0; dt < D / 16; ++dt) v[dt] = *reinterpret_cast<const f32x4*>(x + (int64_t)p * D + dt * 16);
   };
   if (first < n) load(first);
+  unsigned none = kNone;
 #pragma unroll 1
   for (int p = first; p < n; p += step) {
     f32x4 w[D / 16];
@@ -433,6 +441,7 @@ __device__ __forceinline__ void add_parts(const float* ml, const float* x, int f
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) w[dt] = v[dt];
     if (p + step < n) load(p + step);
+    none &= __float_as_uint(c[1]);
     if (c[1] == 0.f) continue;  // (a part without a visible key; its outputs may be anything)
     const float t = fmaxf(m, c[0]), f = __builtin_amdgcn_exp2f(m - t), h = __builtin_amdgcn_exp2f(c[0] - t);
     m = t;
@@ -443,6 +452,7 @@ __device__ __forceinline__ void add_parts(const float* ml, const float* x, int f
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[dt][e] = o[dt][e] * f + w[dt][e] * h;
   }
+  if (lsum[0] == 0.f) lsum[0] = __uint_as_float(__float_as_uint(lsum[0]) & none);
 }
 
 template <int D>
@@ -668,7 +678,7 @@ __device__ __forceinline__ void rows_by_waves(const SharedAttn& a, Item it, char
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
     const int l = anew(), slot = it.first + (w * NS + n) * 16 + (l & 15);
-    if (slot < it.slots) leave<D>(a, it, slot, l >> 4, o[n], m[n], blind >> n & 1 ? 0.f : lsum[n][0]);
+    if (slot < it.slots) leave<D>(a, it, slot, l >> 4, o[n], m[n], blind >> n & 1 ? -0.f : lsum[n][0]);
   }
 }
 
@@ -818,6 +828,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the place is read)
     }
   }
+  if (lim[0] <= it.begin) lsum[0][0] = -0.f;
   const bool finish = it.own && a.finish;
   if (finish) {  // the own part is one workgroup's: the prefix's parts, left by the launch before, join it here, every fourth a wave
     const int l = anew(), slot = it.first + (l & 15), g = l >> 4;
@@ -854,7 +865,7 @@ __device__ __forceinline__ void keys_by_waves(const SharedAttn& a, Item it, char
     } else {
       const int64_t pi = (row * a.nh + head) * a.parts + it.part;
       *reinterpret_cast<f32x4*>(a.po + pi * D + d4 * 4) = j.o;
-      if (d4 == 0) *reinterpret_cast<f32x2*>(a.pml + pi * 2) = f32x2{j.top, j.l};
+      if (d4 == 0) *reinterpret_cast<f32x2*>(a.pml + pi * 2) = f32x2{j.top, j.sum()};
     }
   }
 }
@@ -932,7 +943,7 @@ __global__ __launch_bounds__(256) void attn_shared_join_kernel(const SharedAttn 
     __shared__ __attribute__((aligned(16))) f32x4 so[256];
     __shared__ f32x2 sml[256];
     so[threadIdx.x] = j.o;
-    sml[threadIdx.x] = f32x2{j.top, j.l};
+    sml[threadIdx.x] = f32x2{j.top, j.sum()};
     __syncthreads();
     if (grp > 0) return;
 #pragma unroll

@@ -338,6 +338,28 @@ def test_large_scores_of_many_rows_of_many_heads(size):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nh,nkv,D,owns,qlens", [
+    (8, 2, 128, [40, 30], [1, 1]), (8, 2, 128, [40, 30, 9], [9, 30, 1]), (2, 2, 256, [40, 30, 9], [9, 30, 1]),
+    (48, 1, 64, [400, 30, -20], [1, 1, 1]), (8, 8, 128, [1 + i % 40 for i in range(70)], [1] * 70)])
+def test_keys_of_minus_infinity(dev, nh, nkv, D, owns, qlens):
+    """Keys whose scores are -infinity weigh nothing; a row that sees no others has no softmax, and NaN in its result, not the zeros of
+    a row that sees nothing."""
+    c = _case(dev, nh, nkv, D, 600, owns, qlens=qlens, seed=26)
+    c["q"][:, 3].abs_().clamp_(min=1.0)
+    for h in range(nh):
+        c["q"][:, h * D + 3] = c["q"][:, 3]
+    j = torch.arange(600)
+    c["k"][c["ptab"].long()[j // 16], :, (j % 16).to(dev), 3] = torch.where(j % 3 > 0, float("-inf"), 1.0).bfloat16().to(dev)[:, None]
+    _near(_run(c), c)
+    c["k"][..., 3] = float("-inf")
+    assert _run(c).isnan().all()
+    c["ctx"][1] = 0
+    at = sum(qlens[:1])
+    got = _run(c)
+    assert (got[at:at + qlens[1]] == 0).all() and got[:at].isnan().all() and got[at + qlens[1]:].isnan().all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("qlens", [[1, 1, 1], [3, 20, 5]])
 def test_fp8_rows_of_zeros_and_of_any_scale(dev, qlens):
     """A row whose scale is 0 has its weight all the same; scales from 1e-20 to 1e20 beside each other."""
