@@ -239,6 +239,25 @@ def _need(cond: bool, msg: str):
         raise ValueError(msg)
 
 
+def _rows_meet(a, b, rows: int, ca: int, cb: int) -> bool:
+    """Whether ``rows`` rows of ``ca`` columns of ``a`` and of ``cb`` of ``b``, dense ones, share memory."""
+    if rows == 0:
+        return False
+    pa, pb, ea, eb = a.data_ptr(), b.data_ptr(), a.element_size(), b.element_size()
+    sa, sb, wa, wb = a.stride(0) * ea, b.stride(0) * eb, ca * ea, cb * eb
+    if pa + (rows - 1) * sa + wa <= pb or pb + (rows - 1) * sb + wb <= pa:
+        return False
+    n = np.arange(rows)
+    ra, rb = pa + n * sa, pb + n * sb
+    near = np.searchsorted(rb, ra + wa) - 1  # (the last row of b that begins in front of the end of a's)
+    return bool((rb[np.maximum(near, 0)] + wb > ra)[near >= 0].any())
+
+
+def _same_rows(a, b, rows: int) -> bool:
+    """Whether rows of ``a`` and ``b`` begin in the same places, in the same type."""
+    return a.data_ptr() == b.data_ptr() and a.dtype == b.dtype and (rows <= 1 or a.stride(0) == b.stride(0))
+
+
 def attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx_lens, nh, nkv, D, cu_q, max_qlen, max_own, out):
     """What attn_shared asks of its arguments, on either device: (sequences, fp8 rows, positions that ``max_own`` stands for)."""
     bf16, u8, i32 = torch.bfloat16, torch.uint8, torch.int32
@@ -360,13 +379,14 @@ def adjust_logits_check(logits, ids, lens, prompt_lens, repetition, presence, fr
         _need(out.dim() == 2 and out.shape[0] >= B and out.shape[1] >= V and (out.shape[1] <= 1 or out.stride(1) == 1)
               and (B <= 1 or out.stride(0) >= V) and out.dtype in (logits.dtype, torch.float32),
               "out [B, >= vocab] in the type of logits or fp32, dense rows apart")
+        _need(_same_rows(out, logits, B) or not _rows_meet(out, logits, B, V, V), "out must be logits themselves or share no memory with them")
     return B, V
 
 
 def adjust_logits(logits: torch.Tensor, ids=None, lens=None, prompt_lens=None, repetition=None, presence=None, frequency=None,
                   bias_ids=None, bias=None, mask=None, mask_rows=None, vocab=None, out=None) -> torch.Tensor:
     """The rules in front of the sampler, on rows of logits [B, >= vocab]; returns [B, vocab] in their type, or ``out`` (which may be
-    ``logits`` itself, or fp32). ``ids`` [B, n] are the row's known tokens, ``lens`` [B] how many, ``prompt_lens`` [B] how many of them
+    ``logits`` itself, or fp32; else it shares no memory with the other operands). ``ids`` [B, n] are the row's known tokens, ``lens`` [B] how many, ``prompt_lens`` [B] how many of them
     are its prompt (none without it). A token that is known has its logit divided by ``repetition`` where positive and multiplied where
     not; one that came c > 0 times behind the prompt loses ``c * frequency + presence``; entries (``bias_ids``, ``bias``) [B, m] are added
     in their order (a negative id is no entry); tokens whose bit in the row's mask is clear get -inf: bit t % 32 of word t // 32 of

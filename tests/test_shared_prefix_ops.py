@@ -638,6 +638,44 @@ def test_rules_refusals():
     no("out", x, out=x[:1].expand(2, 64))
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rules_in_place_on_rows_that_are_not_aligned(dev, dtype):
+    c = list(_rules_case(5, 2049, 2051, dtype, 60, 64, 2))
+    x = torch.zeros(5 * 2051 + 8, device=dev).to(dtype)[1:1 + 5 * 2051].view(5, 2051)
+    x.copy_(c[0])
+    got = _adjust(dev, [x, *c[1:]], 2049, out=x)
+    assert got.data_ptr() == x.data_ptr() and torch.equal(x[:, 2049:].cpu(), c[0][:, 2049:])
+    _rules_near(got, c, 2049, dtype)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rules_refuse_a_result_that_overlaps_the_logits_otherwise(dev):
+    """A result that lies over other logits than its own: some would be overwritten before they are read."""
+    buf = torch.zeros(8, 128, device=dev)
+    flat = buf.view(-1)
+    no = lambda x, **kw: pytest.raises(ValueError, ops.adjust_logits, x, **kw).match("out")  # noqa: E731
+    no(flat[:192].view(3, 64), out=flat[8:200].view(3, 64))
+    no(flat[8:200].view(3, 64), out=flat[:192].view(3, 64))
+    no(buf[:4], out=buf[1:5])
+    no(buf[:2, :64], out=flat[:256].view(4, 64)[:2])  # (the same first row, the second over the first's)
+    no(buf[:, 8:72], out=buf[:, 71:])
+    no(buf[:, 8:72], vocab=57, out=buf[:, 64:])
+    half = flat.view(torch.bfloat16)[:256].view(2, 128)
+    no(half, out=flat[:256].view(2, 128))
+    no(half[:1], out=flat[:128].view(1, 128))
+    # beside them, between them, of a row that only one of them has: as good as anywhere
+    buf.copy_(torch.arange(8 * 128).view(8, 128))
+    want = buf.clone()
+    for x, out, kw in ((buf[:, :64], buf[:, 64:], {}), (buf[::2], buf[1::2], {}), (buf[:, 8:72], buf[:, 64:], dict(vocab=56)),
+                       (buf[:3], buf[3:], {}), (buf[:3], buf[:3], {}), (buf[:1], buf[:2], {}), (buf[1:3, :64], buf[:2, 64:], {})):
+        buf.copy_(want)
+        V = kw.get("vocab", x.shape[1])
+        old = x.clone()
+        got = ops.adjust_logits(x, out=out, **kw)
+        assert torch.equal(got, old[:, :V]) and got.data_ptr() == out.data_ptr()
+
+
 # -------------------------------------------------------------------------------------------------------------- logprobs
 def _lp_near(got, want):
     """64 bits' log-softmax: the maximum's difference, an exponential and a logarithm round, and a sum of up to 2^17 terms in
