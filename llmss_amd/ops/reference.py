@@ -295,6 +295,7 @@ def attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_table
     if out is not None:
         _need(out.dtype == bf16 and out.dim() == 2 and out.shape[0] >= T and out.shape[1] >= nh * D and out.stride(1) == 1
               and (T <= 1 or out.stride(0) >= nh * D), "out bf16 [>= T, >= nh * D], rows apart")
+        _need(_same_rows(out, q, T) or not _rows_meet(out, q, T, nh * D, nh * D), "out must be q's own rows or share no memory with them")
     return B, kv8, max_own
 
 
@@ -305,7 +306,7 @@ def attn_shared(q: torch.Tensor, k_cache, v_cache, prefix_table, prefix_len: int
     the pages of ``block_tables[b]``. ``ctx_lens`` [B] counts a sequence's whole context, prefix and new tokens included. Without
     ``cu_q`` row b of ``q`` is the last position of sequence b; with it rows cu_q[b] .. cu_q[b + 1] - 1 are its last positions and each
     sees what is at or before its own. A row whose context is empty gives zeros, rows of no sequence (behind cu_q's last) stay as they
-    are in ``out`` and are not defined without it. ``max_qlen`` and ``max_own`` say how long the longest portion and own part are
+    are in ``out`` and are not defined without it; ``out`` may be ``q``'s own rows and shares no other memory with the operands. ``max_qlen`` and ``max_own`` say how long the longest portion and own part are
     expected to be: they size the work's cuts, longer ones are right all the same."""
     B, _, _ = attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx_lens, nh, nkv, D, cu_q, max_qlen,
                                 max_own, out)

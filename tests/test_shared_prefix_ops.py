@@ -233,6 +233,35 @@ def test_strided_operands(dev):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("nh,nkv,owns,qlens", [
+    (8, 2, [40, 30], [1, 1]), (8, 2, [40, 30, 9], [9, 30, 1]), (8, 8, [1 + i % 40 for i in range(70)], [1] * 70),
+    (24, 8, [9 + i % 40 for i in range(70)], [1 + i % 5 for i in range(70)])])
+def test_attention_in_place_and_beside_its_queries(dev, nh, nkv, owns, qlens):
+    c = _case(dev, nh, nkv, 128, 300, owns, qlens=qlens, seed=27, own_cols=9)
+    want = _run(c)
+    q = c["q"].clone()
+    assert torch.equal(_run(c, out=c["q"])[:, :nh * 128], want) and torch.equal(c["q"][:, nh * 128:], q[:, nh * 128:])
+    c["q"].copy_(q)
+    beside = torch.zeros(q.shape[0], 2 * nh * 128, dtype=torch.bfloat16, device=dev)
+    beside[:, nh * 128:] = q[:, :nh * 128]
+    assert torch.equal(_run(dict(c, q=beside[:, nh * 128:]), out=beside[:, :nh * 128]), want)
+    assert torch.equal(beside[:, nh * 128:], q[:, :nh * 128])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_attention_refuses_a_result_that_overlaps_its_queries_otherwise(dev):
+    c = _case(dev, 4, 2, 64, 33, [3, 30, 18])
+    wide = c["q"].shape[1]
+    flat = torch.zeros(8 * wide, dtype=torch.bfloat16, device=dev)
+    for q, out in ((flat[:3 * wide].view(3, wide), flat[8:8 + 3 * wide].view(3, wide)),
+                   (flat.view(8, wide)[:3], flat.view(8, wide)[1:4]),
+                   (flat.view(8, wide)[:3], flat[:3 * 256].view(3, 256)),
+                   (flat.view(8, wide)[:3, 248:], flat.view(8, wide)[:3])):
+        with pytest.raises(ValueError, match="out"):
+            _run(dict(c, q=q), out=out)
+
+
 def _many(B, several):
     """Own parts and portions of B sequences: idle ones, contexts that end in the prefix, one token to some pages."""
     owns = [(1, 20, 37, None, -30, 90, 64, 16, 33, 5)[i % 10] for i in range(B)]
