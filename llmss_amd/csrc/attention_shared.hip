@@ -95,6 +95,8 @@ __device__ __forceinline__ int slot_limit(const SharedAttn& a, const Item& it, i
   return it.own ? min(max(n - a.P, 0), a.own_cap) : min(n, a.P);
 }
 
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (that m0, which `to_lds` names as changed, is none of the registers the compiler gives out)
 // Where the cache rows of a tile of 16 KT keys lie, in bytes. Pages of 16, 32, 64 .. positions (BY16): a lane asks for the page of one
 // run of 16 keys, a tile ahead (a vector load, which the wait in front of the next tile covers: a scalar one would have the reads of
 // LDS wait for it); a run's address is formed in scalar registers, a lane adds 32 bits. Others: each row asks for its own page where
@@ -138,21 +140,22 @@ struct Rows {
     else return *reinterpret_cast<const V*>((const char*)cache + alone(kv0 + 16 * run + r) + more);
   }
   // 16 bytes a lane from memory into LDS (lane l at `at` + 16 l, the same `at` in every lane). Through inline assembly, so that the compiler does not hold reads
-  // of other places in LDS back until it has landed: every use stands behind a wait for vmcnt(0) of its own.
+  // of other places in LDS back until it has landed: every use stands behind a wait for vmcnt(0) of its own. The compiler does not see into it: it is told
+  // that m0 changes, and the base is written again by a scalar move (which also is what has to stand between a write of m0 and the load), as one that a
+  // vector instruction wrote (a spilled one's v_readlane) may not be read by a load within five instructions.
   __device__ __forceinline__ void to_lds(const char* p, unsigned off, unsigned at) const {  // (all of a run's rows: p the run's, off a lane's)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b64 %0, %0\n\tglobal_load_lds_dwordx4 %1, %0" : "+s"(p) : "v"(off), "s"(at) : "memory", "m0");
   }
   __device__ __forceinline__ void to_lds(const void* cache, int64_t run_at, int kv0, int run, int r, unsigned more, unsigned at) const {
     if constexpr (BY16) {
-      const char* p = (const char*)cache + run_at;
-      const unsigned off = row_at(kv0, run, r) + more;
-      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p), "s"(at) : "memory");
+      to_lds((const char*)cache + run_at, row_at(kv0, run, r) + more, at);
     } else {
       const char* p = (const char*)cache + alone(kv0 + 16 * run + r) + more;
-      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory");
+      asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory", "m0");
     }
   }
 };
+#pragma clang diagnostic pop
 
 // Has the compiler wait for what was loaded into x: a first use inside a loop would be waited for in every turn, and with it
 // for the loads into LDS that it does not count.

@@ -7,6 +7,8 @@ the sum, and the result once; with A = sum_j p_j |v_j| that is at most 2^-8 (2 A
 fp32 products of scores (128 products of numbers around 1 and their sum: 2^-24 * 128 * 4 in a score, far below). fp32 results:
 each operation 2^-24 of its terms."""
 import math
+import pathlib
+import re
 
 import pytest
 import torch
@@ -231,6 +233,23 @@ def test_strided_operands(dev):
     tables[:, 4:4 + c["bt"].shape[1]] = c["bt"]
     got = _run(dict(c, q=wide[:, 64:], bt=tables[:, 4:4 + c["bt"].shape[1]]))
     assert torch.equal(got, want)
+
+
+def test_loads_into_lds_by_assembly_say_what_they_change():
+    """The compiler sees into no string: a statement that writes m0 names it as changed, and a memory instruction in it takes its scalar
+    address from a move of the same statement (the compiler keeps the distance from a vector write of it for its own instructions only)."""
+    csrc = pathlib.Path(ops.__file__).parents[1] / "csrc"
+    found = 0
+    for f in sorted(csrc.glob("*.hip")) + sorted(csrc.glob("*.h")):
+        for code, rest in re.findall(r'asm volatile\(("(?:[^"\\]|\\.)*")\s*:(.*?)\);', f.read_text(), re.S):
+            if "global_load_lds" in code:
+                found += 1
+                outputs = len(re.findall(r'"[=+]', rest))
+                base = re.search(r"global_load_lds\w+ %\d, (?:%(\d)|off)", code)
+                assert base, code
+                assert base[1] is None or int(base[1]) < outputs, f"{f.name}: {code}"
+            assert not re.search(r"\w m0,", code) or '"m0"' in rest, f"{f.name}: {code}"
+    assert found >= 2
 
 
 @pytest.mark.parametrize("dev", DEVICES)
