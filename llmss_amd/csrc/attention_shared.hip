@@ -1059,7 +1059,7 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
   a.bs = bs;
   a.shift = __builtin_ctz(bs);
   const int64_t page_bytes = (int64_t)nkv * bs * (kv8 ? D + kTail : 2 * D);
-  if (page_bytes > INT_MAX) throw std::runtime_error("attn_shared: pages of 2 GiB and more");
+  if (page_bytes > INT_MAX) throw std::invalid_argument("attn_shared: pages of 2 GiB and more");
   a.page_bytes = (unsigned)page_bytes;
   a.pages = pages;
   a.P = P;
@@ -1080,7 +1080,9 @@ void launch_attn_shared(const void* q, int64_t q_stride, const void* kc, const v
   const int64_t pre = (int64_t)p.pre_tiles * nkv * p.pre_split, own = (int64_t)B * nkv * p.own_tiles * p.own_split;
   const int together = parts > 12 ? 1024 / D : 1;  // (see the join kernel)
   const int64_t join = ((int64_t)T * nh * (D / 4) * together + 255) / 256;
-  if (pre + own > INT_MAX || join > INT_MAX || (int64_t)T * (nh / nkv) > INT_MAX / 2) throw std::runtime_error("attn_shared: too many rows");
+  constexpr int64_t kMostGroups = UINT32_MAX / 256;  // (a launch has fewer than 2^32 threads)
+  if (pre + own > kMostGroups || join > kMostGroups || (int64_t)T * (nh / nkv) > INT_MAX / 2)
+    throw std::invalid_argument("attn_shared: too many rows");
   // one launch for both parts where they take the same form; else the own parts', which follow, join the prefix's results themselves
   // (each is one workgroup's: there are 512 pairs or more)
   const bool apart = p.own_few && !p.pre_few && pre > 0;

@@ -265,6 +265,7 @@ def attn_shared(q, k_cache, v_cache, prefix_table, prefix_len, block_tables, ctx
     if T == 0 or B == 0:
         return y
     C = lib()
+    max_qlen = min(max_qlen, T)
     parts = C.attn_shared_parts(T, B, nh, nkv, D, prefix_len, max_qlen, max_own, kv8)
     ws = q.new_empty(T * nh * parts * (D + 2), dtype=torch.float32)
     nb, _, bs, _ = k_cache.shape

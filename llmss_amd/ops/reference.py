@@ -276,9 +276,11 @@ def attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_table
     _need(block_tables.dtype == i32 and block_tables.dim() == 2 and (block_tables.shape[1] <= 1 or block_tables.stride(1) == 1),
           "block_tables int32 [B, pages], dense rows")
     _need(ctx_lens.dtype == i32 and ctx_lens.dim() == 1 and ctx_lens.is_contiguous(), "ctx_lens int32 [B]")
-    _need(isinstance(prefix_len, int) and 0 <= prefix_len <= prefix_table.numel() * bs,
-          "prefix_len must be a number between 0 and what prefix_table holds")
+    _need(nkv * bs * cs[3] * k_cache.element_size() < 1 << 31, "pages of 2 GiB and more")
+    _need(isinstance(prefix_len, int) and 0 <= prefix_len <= min(prefix_table.numel() * bs, (1 << 30) - 1),
+          "prefix_len must be a number between 0 and what prefix_table holds, and below 2 ** 30")
     T = q.shape[0]
+    _need(T * (nh // nkv) < 1 << 30, "2 ** 30 rows of a key head and more")
     if cu_q is None:
         B = T
         _need(max_qlen == 1, "several tokens a sequence need cu_q")
@@ -292,6 +294,7 @@ def attn_shared_check(q, k_cache, v_cache, prefix_table, prefix_len, block_table
     if max_own is None:
         max_own = room
     _need(isinstance(max_own, int) and 0 <= max_own <= room, "max_own must be between 0 and what a row of block_tables holds")
+    max_own = min(max_own, (1 << 30) - 1)
     if out is not None:
         _need(out.dtype == bf16 and out.dim() == 2 and out.shape[0] >= T and out.shape[1] >= nh * D and out.stride(1) == 1
               and (T <= 1 or out.stride(0) >= nh * D), "out bf16 [>= T, >= nh * D], rows apart")

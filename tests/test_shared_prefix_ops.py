@@ -456,6 +456,45 @@ def test_rows_of_logits_past_32_bits():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_attention_refuses_what_passes_32_bits(dev):
+    """Places in a cache, rows and positions that the kernels' numbers do not hold: ValueError, as for everything that is not taken,
+    before anything is allocated. Hints may be of any size."""
+    i32 = dict(dtype=torch.int32, device=dev)
+    q = torch.randn(1, 192, generator=torch.Generator().manual_seed(1)).bfloat16().to(dev)
+    k = torch.randn(3, 1, 2048, 64, generator=torch.Generator().manual_seed(2)).bfloat16().to(dev)
+    far = torch.zeros(1 << 20, **i32)  # (2^31 positions of one page)
+    near = torch.tensor([[1]], **i32)
+    ctx = torch.tensor([3000], **i32)
+    cu = torch.tensor([0, 1], **i32)
+
+    def call(q=q, k=k, ptab=near[0], prefix=2048, bt=near, **kw):
+        return ops.attn_shared(q, k, k, ptab, prefix, bt, ctx, 1, 1, 64, 0.1, **kw)
+
+    def no(match, **kw):
+        with pytest.raises(ValueError, match=match):
+            call(**kw)
+
+    no("pages", k=torch.empty(1, 1, 1 << 24, 64, dtype=torch.bfloat16, device=dev))
+    no("rows", q=q.expand(1 << 30, 192), cu_q=cu)
+    no("prefix_len", ptab=far, prefix=1 << 31)
+    no("prefix_len", ptab=far, prefix=1 << 30)
+    for got in (call(), call(bt=torch.cat([near, far[None, 1:]], 1)), call(bt=torch.cat([near, far[None, 1:]], 1), max_own=(1 << 31) - 1),
+                call(cu_q=cu, max_qlen=1 << 40), call(cu_q=cu, max_qlen=1 << 30)):
+        _near(got, dict(q=q, k=k, v=k, ptab=near[0], prefix=2048, bt=near, ctx=ctx, qlens=[1], nh=1, nkv=1, D=64, bs=2048, scale=0.1))
+
+
+def test_more_workgroups_than_a_launch_takes_are_refused():
+    """At the native entry, which looks at them before it touches anything."""
+    from llmss_amd import _native
+
+    C = _native()
+    T = 1 << 26  # (four rows a workgroup of the joining launch: 2^32 threads)
+    parts = C.attn_shared_parts(T, 1, 1, 1, 256, 0, 1, 1, False)
+    with pytest.raises(ValueError, match="too many rows"):
+        C.attn_shared(0, 256, 0, 0, 1, 0, 0, 0, 1, 1, 0, 0, 0, 256, 0, parts, T, 1, 1, 1, 256, 16, 1, 1, 0.1, False, 0)
+
+
 def test_attention_refusals():
     c = _case("cpu", 4, 2, 64, 33, [3, 30, 18])
 
