@@ -863,6 +863,87 @@ def test_the_likeliest_of_sorted_rows():
         assert torch.equal(ids, torch.sort(x, dim=-1, descending=True, stable=True)[1][:, :n])
 
 
+def _unusual_rows(V, dtype):
+    """Rows that strain the search for the likeliest, for cuts of some thousand tokens: (rows, tokens)."""
+    g = torch.Generator().manual_seed(V)
+    nan, inf = float("nan"), float("inf")
+    run = V // 16
+    x = torch.randn(14, V, generator=g) * 3
+    up = torch.arange(V, dtype=torch.float32) * 1e-3
+    x[0], x[1], x[2], x[3], x[4] = up, up.flip(0), (torch.arange(V) % 2).float(), 2.0, -inf
+    few = torch.randperm(V, generator=g)
+    x[5, few[3:]] = nan  # three numbers among NaN, and forty
+    x[6, few[40:]] = nan
+    x[7, 2 * run:5 * run] = nan  # whole runs of NaN, of -inf, all but one of -inf
+    x[8, 2 * run:5 * run] = -inf
+    x[9, :9 * run] = -inf
+    x[9, 11 * run:] = -inf
+    x[10] = nan
+    x[11] = torch.finfo(dtype).min
+    x[11, few[:5]] = torch.arange(5).float()
+    x[12, V // 2] = inf
+    x[13] = torch.where(x[13] > 0, 0.0, -0.0)
+    tok = torch.randint(0, V, (14,), generator=g)
+    tok[5], tok[9], tok[11], tok[12] = few[1], 10 * run, few[2], V // 2
+    return x.to(dtype), tok
+
+
+def _likeliest_plain(x, n):
+    """The n likeliest of each row: falling values, the lower token first, no NaN; -1 where there are fewer."""
+    ids = torch.full((x.shape[0], n), -1, dtype=torch.int64)
+    for b in range(x.shape[0]):
+        at = torch.nonzero(~x[b].isnan())[:, 0]
+        order = at[torch.sort(x[b][at].double(), descending=True, stable=True)[1]][:n]
+        ids[b, :order.numel()] = order
+    return ids
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("wide", [0, 1])  # (odd strides: rows that are not aligned)
+@pytest.mark.parametrize("B,V", [(14, 65537), (14, 131071), (300, 50257)])
+def test_log_probabilities_in_two_launches(B, V, wide, dtype):
+    """Vocabularies and batches whose rows are several workgroups', with up to 64 likeliest: ordinary rows and unusual ones."""
+    from llmss_amd.ops import hip
+
+    assert hip.lib().logprobs_runs(B, V) > 1
+    odd, tok = _unusual_rows(V, dtype)
+    cols = V + wide if wide else (V + 7) // 8 * 8
+    x = torch.zeros(B, cols, dtype=dtype, device="cuda")[:, :V]
+    x[:14] = odd.cuda()
+    if B > 14:
+        x[14:] = (torch.randn(B - 14, V, generator=torch.Generator(device="cuda").manual_seed(B), device="cuda") * 4).to(dtype)
+        tok = torch.cat([tok, torch.randint(0, V, (B - 14,), generator=torch.Generator().manual_seed(B))])
+    at = torch.arange(B)
+    want = torch.log_softmax(x.double(), -1).cpu()
+    want[4] = float("-inf")
+    rank = 1 + (x.double() > x.double()[at, tok.cuda()][:, None]).sum(-1).cpu()
+    every = _likeliest_plain(x.cpu(), 64)
+    for n in (0, 1, 20, 33, 64):
+        lp, r, ids, top = (t.cpu() for t in ops.token_logprobs(x, tok.cuda(), n))
+        assert torch.equal(ids, every[:, :n]) and torch.equal(r, rank) and top.shape == (B, n)
+        for got, w in ((lp, want[at, tok]), (top, torch.where(ids < 0, float("nan"), want.gather(1, ids.clamp(min=0))))):
+            assert torch.equal(got.isnan(), w.isnan())
+            _lp_near(got[~got.isnan()], w[~w.isnan()])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("V", [300, 9001, 20001, 65536])
+def test_log_probabilities_of_unusual_rows(dev, V):
+    """The same rows where each is one workgroup's, and by the definition."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x, tok = _unusual_rows(V, dtype)
+        want = torch.log_softmax(x.double(), -1)
+        want[4] = float("-inf")
+        for n in (0, 1, 20, 33, 64):
+            lp, r, ids, top = (t.cpu() for t in ops.token_logprobs(x.to(dev), tok.to(dev), n))
+            assert torch.equal(ids, _likeliest_plain(x, n))
+            assert torch.equal(r, 1 + (x.double() > x.double()[torch.arange(14), tok][:, None]).sum(-1))
+            for got, w in ((lp, want[torch.arange(14), tok]), (top, torch.where(ids < 0, float("nan"), want.gather(1, ids.clamp(min=0))))):
+                assert torch.equal(got.isnan(), w.isnan())
+                _lp_near(got[~got.isnan()], w[~w.isnan()])
+
+
 def test_log_probabilities_refusals():
     x = torch.zeros(2, 64)
     t = torch.zeros(2, dtype=torch.int64)
