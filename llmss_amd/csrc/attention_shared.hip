@@ -24,14 +24,15 @@
 // Together they make three kinds of call (`shared_plan`): both parts in one launch of either form and a launch that joins, or the prefix
 // by rows and then own parts by keys, which join the prefix's results themselves.
 //
-// Measured: 128 rows of 64 heads in 8 groups behind 16381 positions 84 us for the prefix (820 TFLOP/s; 256 rows
-// behind 16384 135 us, 1.0 PFLOP/s), 38 for own parts of up to 500; 64 rows of 32 heads behind 2048 positions 13.5 + 28 (own parts at
-// 4 TB/s); 16 heads of 256 with 24 questions behind 1777 positions 101 (540 TFLOP/s, near what one group a fragment allows) + 16 for the
+// Measured: 128 rows of 64 heads in 8 groups behind 16381 positions 83 us for the prefix (830 TFLOP/s; 256 rows
+// behind 16384 135 us, 1.0 PFLOP/s), 39 for own parts of up to 500; 64 rows of 32 heads behind 2048 positions 12 + 28 (own parts at
+// 4 TB/s); 16 heads of 256 with 24 questions behind 1777 positions 101 - 106 (530 TFLOP/s, near what one group a fragment allows) + 17 for the
 // join.
 //
-// Keys that a slot does not see weigh nothing whatever lies there: scores are replaced, not multiplied; rows past the last visible
-// key are never loaded (a visible one is, again); and where a tile that is masked for some slots holds values that are not finite,
-// they are kept from the slots that do not see them (see `add_values`).
+// Keys that a slot does not see weigh nothing whatever lies there: scores are replaced, not multiplied; and where a tile that is masked
+// for some slots holds values that are not finite, they are kept from the slots that do not see them (see `add_values`). In place of rows past
+// the last visible key a row that the cache has is loaded: the last visible one again or, by keys, one of a page that was asked for before
+// the length was known.
 // fp8 cache rows: e4m3 numbers are exact in bf16, a row's scale multiplies its score and its weight.
 #include "common.h"
 
@@ -981,18 +982,20 @@ double cut_prefix(Plan& p, int ns, int64_t slots, int nkv, int D, int P) {
   return rounds * p.pre_keys / 64 * (ns == 2 ? 3.3 : 2.0) + 2.0 * slots * nkv * (D + 2) * 4 * p.pre_split / 4.5e6;
 }
 
-// Which form takes what:
-//  up to 16 slots in the whole batch: both parts by keys (one row of 32 heads in 8 groups behind 2000 positions 13.5 us, the prefix by
-//   rows 18.9; 4 rows behind 30000 27.2 and 33.6; 2 rows of fp8 behind 16000 16.8 and 29.0).
+// Which form takes what (the calls among others; heads of 128 as 32 in 8 groups where nothing else is said):
+//  up to 16 slots in the whole batch: both parts by keys (one row behind 2000 positions 9.4 us from a captured graph, the prefix by rows
+//   11.5, either 15 with the host's steps; 2 rows behind 16000 19.5 and 21.7, of fp8 16.9 and 21.0; 4 rows behind 30000 27.9 and 27.0, of fp8
+//   22.4 and 25.8).
 //  own parts by keys in a launch of their own, after the prefix's, where up to 16 slots a sequence and at least 512 (sequence, key
-//   head) pairs fill the chip: each pair is then one workgroup's, and no third launch joins (64 rows of 32 key heads behind 2048 39.1 us,
-//   in one launch with the prefix by rows 43.0; 128 rows of 8 behind 16381 115 and 124; 100 fp8 rows of 8 behind 2000 30.7 and 37.2).
+//   head) pairs fill the chip: each pair is then one workgroup's, and no third launch joins (64 rows of 32 key heads behind 2048 39.7 us,
+//   in one launch with the prefix by rows 42.4, of fp8 34.9 and 43.4; 128 rows of 64 heads in 8 behind 16381 119 and 122, of fp8 150 and 149; 100
+//   rows behind 2000 29.4 and 29.6, of fp8 29.0 and 32.6).
 //   Not where own parts are long beside the prefix, which then fill its gaps (64 rows of 8, 2000 and up to 3000 positions: 117 us apart,
 //   112 together), and not for heads of 64 (equal, or 69 together and 74) and of 256 (30 and 40: by keys two workgroups share a compute
 //   unit, not four).
 //  everything else by rows in one launch (fewer pairs: 60 rows of one key head behind 4000 18.0 us, apart 25.8; 33 rows of 48 heads on
 //   one key head behind 7990 26.1 and 31.7).
-//  no prefix: own parts of up to 16 slots by keys (64 rows of 8 key heads of up to 500 18.7 us, by rows 19.4; fp8 24.1 and 35.0).
+//  no prefix: own parts of up to 16 slots by keys (64 rows of up to 500 19.5 us, by rows 19.9; fp8 17.4 and 23.2).
 // Own parts are cut until there are 256 workgroups by rows beside the prefix's (20 rows of 8 key heads with 4 tokens each 24.1 us, with 512
 // 27.6, with 2048 33.3) and 512 by keys (2 rows of 8 with up to 8000 positions 15.5, with 256 19.6, with 2048 15.4).
 Plan shared_plan(int T, int B, int nkv, int G, int D, int P, int max_qlen, int max_own, bool kv8) {

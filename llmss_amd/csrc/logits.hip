@@ -12,7 +12,8 @@
 // biases a row cost 256 x 131071 fp32 logits 27 us beside 48, written once more 6). Integer counts, and biases summed in the order of the
 // list: the result does not depend on the order in which threads run.
 // 256 rows of 131071 fp32 logits 48 us as they are (5.6 TB/s), with up to 8000 known tokens, 300 biases and a mask 67; 64 of 50257 in bf16 with
-// up to 1000 known tokens 9.6, one of 32000 3.9, a chain of waits.
+// up to 1000 known tokens 9.6, one of 32000 3.9, a chain of waits. Rows that do not start on 16 bytes go a token at a time: 64 of 50257 in bf16
+// 12.4 us, 256 31.7 (aligned 9.5, 21.8).
 #include "common.h"
 
 #include <type_traits>

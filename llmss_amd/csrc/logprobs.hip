@@ -9,8 +9,9 @@
 // the value, so no two are equal: where a run of equal logits has more than the list takes, the search goes on over all bits. A NaN
 // counts as no candidate, and makes its row's log-probabilities NaN; a row of nothing but -inf has log-probabilities of -inf. Few rows of
 // ordinary vocabularies take one launch, a workgroup a row.
-// One row of 32000 bf16 tokens 8.0 us, a chain of waits (tokens, maximum, sum, search, list); 64 of 50257 13.9, as they are one compute
-// unit's each; 256 of 131071 fp32 tokens with 20 likeliest 28.5 + 6.5, the first 4.7 TB/s.
+// One row of 32000 bf16 tokens 8.0 us, a chain of waits (tokens, maximum, sum, search, list); 64 of 50257 13.3, as they are one compute
+// unit's each; 256 of 131071 fp32 tokens with 20 likeliest 28.6 + 6.5, the first 4.7 TB/s. Rows that do not start on 16 bytes are read a token
+// at a time: 64 of 50257 bf16 tokens 23.5 us, 256 24.9 (aligned 13.3, 16.4).
 #include "common.h"
 
 #include <type_traits>
@@ -337,9 +338,12 @@ constexpr int kNT = 256, kPacks = 4;
 constexpr int kAlone = 1024;  // threads where a row is one run
 
 // Whether a row is one workgroup's, of 1024 threads with 2, 4 or 8 packs: while there is a compute unit for each (two workgroups
-// with 2 packs share one). It saves the second launch and the partial results: with a call's host steps 32000 tokens of one row 10.9 us
-// and 14.3 in two launches, 256 rows of 50257 16.9 and 21.2, 512 of 9000 13.0 and 15.0; beyond, 300 rows of 32000 17.4 and 16.3, 512 of
-// 50257 28.8 and 26.4, 1000 of 16000 23.7 and 22.4.
+// with 2 packs share one). It saves the second launch and the partial results. The calls in one launch and in two, with the host's steps
+// and from a captured graph, bf16: one row of 32000 11.7 and 15.6 us, captured 8.2 and 11.0; 128 rows of 32000 11.4 and 15.7, captured 10.2
+// and 11.9; 512 of 9000 13.1 and 15.9, captured 12.7 and 14.1; 256 of 50257 16.4 and 19.6, captured 16.3 and 19.4; beyond, 300 rows of 32000
+// 18.6 and 17.1, captured 18.4 and 16.3, 512 of 50257 29.7 and 27.3, captured 29.9 and 27.2. Few rows of 8 packs are the exception: 64 of
+// 50257 take 13.9 us and 15.7 with the host's steps, but 13.3 and 12.1 captured (8 rows 12.4 and 11.4): the second launch costs a graph
+// less than three quarters of the chip.
 bool alone(int B, int V) { return V <= kAlone * 8 * 2 ? B <= 512 : V <= kAlone * 8 * 8 && B <= 256; }
 
 // Keys that a run's list holds: several times what is found as a rule, and what the exact way may need.
